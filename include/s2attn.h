@@ -272,6 +272,28 @@ int s2attn_backward_saved_noalloc(const void *k, const void *v, const void *q, c
                                   const s2attn_shape *shape, void *stream);
 
 /*
+ * Differential attention: the difference of two softmax maps over the same neighborhood, with one learned weight per head.  It has no
+ * counterpart in the reference.  Tensors, plan, directions and strides as for s2attn_forward, except that a head's row of k and q (and dk, dq)
+ * holds two vectors: shape->ck is the channels of ONE of them (1 to 256), rows are num_heads * 2 * ck long, (q1 | q2) of head 0 first; cv
+ * up to 512.  Unpacked tensors (point strides) are taken by every shape.  lam: num_heads numbers of type lam_dtype in device memory.
+ *   y = sum_j (p1_j - lam p2_j) v_j,   pi_j = exp(qi.ki_j) quad_weights[hi_j] / sum_l exp(qi.ki_l) quad_weights[hi_l]
+ * y2 (second map's output, packed, storage dtype) and lse (float[2] per batch entry, head and output point) are what the backward needs:
+ * both or neither (inference).  A point that sees nothing, by psi or because all it sees has weight zero, has y = 0 and neither gives nor
+ * takes a gradient.  What is not finite reaches the points that see it, as arithmetic on each point's neighbors has it, and no other.
+ *
+ * Backward: writes dq, dk and dv (both, or neither if null) and dlam (of lam_dtype; may be null), every element, without atomics: results are
+ * the same in every run.  workspace: s2attn_diff_backward_workspace_bytes(shape) of device memory, 16-byte aligned; calls that overlap
+ * need one each.
+ */
+int s2attn_diff_forward(const void *k, const void *v, const void *q, const void *lam, int lam_dtype, const float *quad_weights, void *y, void *y2, float *lse,
+                        const s2attn_plan *plan, const s2attn_shape *shape, void *stream);
+
+int64_t s2attn_diff_backward_workspace_bytes(const s2attn_shape *shape);
+
+int s2attn_diff_backward(const void *k, const void *v, const void *q, const void *lam, int lam_dtype, const void *dy, const void *y, const void *y2, const float *lse,
+                         const float *quad_weights, void *dk, void *dv, void *dq, void *dlam, void *workspace, const s2attn_plan *plan, const s2attn_shape *shape, void *stream);
+
+/*
  * Layout conversion.  Replace attention_kernels::permute_to_nhwc / permute_to_nchw
  * (attention_interface.cpp:85-86; CUDA kernels attention_cuda_utils.cuh:417-576).
  * Pure element moves; elem_size is 2, 4 or 8 bytes.  dst must not alias src.

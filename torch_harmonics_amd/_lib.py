@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(_HERE, "libs2attn.so")
 TORCH_LIB_PATH = os.path.join(_HERE, "_C.so")  # libtorch registration of the operators (csrc/s2attn_torch.cpp)
 
 S2ATTN_F32, S2ATTN_BF16, S2ATTN_F16 = 0, 1, 2
-ABI_VERSION = 14
+ABI_VERSION = 15
 NOALLOC_SCRATCH_BYTES = 64 * 1024 * 1024
 
 _vp = ctypes.c_void_p
@@ -142,6 +142,9 @@ SYMBOLS = {
     "s2attn_backward": (_int, [_vp] * 9 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
     "s2attn_backward_dq": (_int, [_vp] * 7 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
     "s2attn_backward_dkdv": (_int, [_vp] * 8 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
+    "s2attn_diff_forward": (_int, [_vp] * 4 + [_int] + [_vp] * 4 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
+    "s2attn_diff_backward_workspace_bytes": (_i64, [ctypes.POINTER(ShapeStruct)]),
+    "s2attn_diff_backward": (_int, [_vp] * 4 + [_int] + [_vp] * 10 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
     "s2attn_permute_to_nhwc": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _int, _vp]),
     "s2attn_permute_to_nchw": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _int, _vp]),
     "s2attn_pack_k16": (_int, [_int, _int]),
@@ -219,7 +222,7 @@ _torch_ops_loaded = False
 
 def load_torch_ops() -> None:
     """Loads _C.so, whose static initialisers register attention_kernels::{forward, backward, permute_to_nhwc, permute_to_nchw}
-    and s2attn_kernels::{forward_lse, backward_saved} with the dispatcher; raises if it is not built."""
+    and s2attn_kernels::{forward_lse, backward_saved, differential_*, ...} with the dispatcher; raises if it is not built."""
     global _torch_ops_loaded
     if _torch_ops_loaded:
         return

@@ -36,11 +36,11 @@
 
 #include "s2attn_internal.h"
 
-// This file is compiled six times (see the Makefile), so that the groups of kernel instantiations build side by
+// This file is compiled seven times (see the Makefile), so that the groups of kernel instantiations build side by
 // side: S2_PART 1 = everything but the launchers of the 16-longitude matrix-core families, 2 = the 16-bit family
 // (s2attn_h16.hpp), 3 = the fp32 family (s2attn_m32.hpp), 4 = its ring-step kernels for 16-bit storage, 5 = the split-product family
 // (s2attn_s16.hpp), 6 = its ring steps
-// (s2attn_s16_ring.hpp).  S2_PART 0 (the default) is the whole library in one unit.
+// (s2attn_s16_ring.hpp), 7 = differential attention one point at a time (s2attn_diff.hpp).  S2_PART 0 (the default) is the whole library in one unit.
 #ifndef S2_PART
 #define S2_PART 0
 #endif
@@ -61,7 +61,7 @@ int s2attn_fail(int code, const char *fmt, ...)
 }
 
 extern "C" const char *s2attn_last_error(void) { return g_err; }
-extern "C" int s2attn_abi_version(void) { return 14; }
+extern "C" int s2attn_abi_version(void) { return 15; }
 #endif
 
 namespace s2 {
@@ -2283,6 +2283,7 @@ template <typename T> __global__ __launch_bounds__(64) void dkdv_mfma_kernel(con
 #include "s2attn_m32.hpp"
 #include "s2attn_s16.hpp"
 #include "s2attn_s16_ring.hpp"
+#include "s2attn_diff.hpp"
 
 // ---------------------------------------------------------------------------------
 // layout permutes: batched 2-D transpose [R, S] -> [S, R] through a 64x65 LDS tile
@@ -2321,6 +2322,7 @@ template <typename T, int D, bool PAD> int launch_s16(Which which, const Args &a
 template <typename T, int D, bool PAD, int MODE> int launch_ring_s16(const Args &a0, hipStream_t stream);
 template <int D, int MODE, typename T> int launch_ring_m32(const Args &a0, hipStream_t stream);
 template <int D, bool WRITE, typename T> int launch_ring_pass2_m32(const Args &a0, hipStream_t stream);
+template <typename T> int launch_diff_points(Which which, const DArgs &a, hipStream_t stream);
 
 #if S2_PART == 0 || S2_PART == 2
 // 16-bit matrix-core kernels: bf16 / fp16 storage, head dim D, equal longitude counts, 16-byte aligned tensors.  The
@@ -2559,6 +2561,34 @@ template int launch_ring_m32<128, 1, f16_t>(const Args &, hipStream_t);
 template int launch_ring_m32<128, 2, f16_t>(const Args &, hipStream_t);
 #endif
 
+#if S2_PART == 0 || S2_PART == 7
+// differential attention, one point at a time
+template <typename T, int N> int launch_diff_points_n(Which which, const DArgs &a, hipStream_t stream)
+{
+    const long points = (which == DKDV ? (a.dk ? (long)a.Hi * a.Wi : 0) : (long)a.Ho * a.Wo) * a.B * a.nh;
+    const int lam_blocks = which == DKDV && a.dlam ? a.nh : 0;
+    const long nblocks = lam_blocks + std::min((points + DPT - 1) / DPT, 1L << 23);
+    if (nblocks == 0) return S2ATTN_OK;
+    void (*const kern)(const DArgs, int, long) = which == FWD ? diff_points_kernel<T, N, FWD> : which == DQ ? diff_points_kernel<T, N, DQ> : diff_points_kernel<T, N, DKDV>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(64 * DPT), 0, stream, a, lam_blocks, points);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return s2attn_fail(S2ATTN_E_LAUNCH, "kernel launch: %s", hipGetErrorString(e));
+    return S2ATTN_OK;
+}
+template <typename T> int launch_diff_points(Which which, const DArgs &a, hipStream_t stream)
+{
+    const int c = std::max(a.dk_, a.dv_);
+    if (c <= 32) return launch_diff_points_n<T, 2>(which, a, stream);
+    if (c <= 64) return launch_diff_points_n<T, 4>(which, a, stream);
+    if (c <= 128) return launch_diff_points_n<T, 8>(which, a, stream);
+    return launch_diff_points_n<T, 32>(which, a, stream);
+}
+#endif
+#if S2_PART == 7
+template int launch_diff_points<float>(Which, const DArgs &, hipStream_t);
+template int launch_diff_points<bf16_t>(Which, const DArgs &, hipStream_t);
+template int launch_diff_points<f16_t>(Which, const DArgs &, hipStream_t);
+#endif
 } // namespace s2
 
 #if S2_PART <= 1
@@ -3350,6 +3380,82 @@ extern "C" int s2attn_backward_saved_noalloc(const void *k, const void *v, const
     // the dq pass writes both statistics of every (batch, head, output point) before the dk/dv pass reads them, so
     // nothing of a previous call's contents is ever read and nothing needs clearing
     return s2attn_backward_saved(k, v, q, dy, y, lse, quad_weights, dk, dv, dq, ws, plan, shape, stream);
+}
+
+// ---------------------------------------------------------------------------------
+// differential attention
+// ---------------------------------------------------------------------------------
+namespace {
+// The shape as the kernels take it: a head's row of q and k holds the channels of both maps.
+int diff_shape(s2attn_shape &sh, const s2attn_shape *shape)
+{
+    if (!shape) return s2attn_fail(S2ATTN_E_INVALID, "shape is null");
+    sh = *shape;
+    if (sh.ck < 1 || sh.ck > 256) return s2attn_fail(sh.ck < 1 ? S2ATTN_E_INVALID : S2ATTN_E_UNSUPPORTED, "differential attention takes maps of 1 to 256 channels, got %d", sh.ck);
+    sh.ck *= 2;
+    return check_shape(&sh);
+}
+int diff_args(DArgs &a, const void *k, const void *v, const void *q, const void *lam, int lam_dtype, const float *quad_weights, const s2attn_plan *plan, const s2attn_shape *shape)
+{
+    s2attn_shape sh;
+    int rc = diff_shape(sh, shape);
+    if (rc != S2ATTN_OK) return rc;
+    if (!k || !v || !q || !lam || !quad_weights) return s2attn_fail(S2ATTN_E_INVALID, "null tensor pointer");
+    if (lam_dtype != S2ATTN_F32 && lam_dtype != S2ATTN_BF16 && lam_dtype != S2ATTN_F16) return s2attn_fail(S2ATTN_E_INVALID, "unknown dtype code %d of lam", lam_dtype);
+    rc = check_plan(plan, &sh);
+    if (rc != S2ATTN_OK) return rc;
+    fill_args(a, plan, &sh, quad_weights);
+    a.k = k, a.v = v, a.q = q, a.lam = lam, a.lam_dtype = lam_dtype;
+    return S2ATTN_OK;
+}
+template <typename T> int launch_diff_t(Which which, DArgs &a, hipStream_t stream)
+{
+    return launch_diff_points<T>(which, a, stream);
+}
+int launch_diff(Which which, DArgs &a, int dtype, hipStream_t stream)
+{
+    if (dtype == S2ATTN_F32) return launch_diff_t<float>(which, a, stream);
+    return dtype == S2ATTN_BF16 ? launch_diff_t<bf16_t>(which, a, stream) : launch_diff_t<f16_t>(which, a, stream);
+}
+} // namespace
+
+extern "C" int s2attn_diff_forward(const void *k, const void *v, const void *q, const void *lam, int lam_dtype, const float *quad_weights, void *y, void *y2, float *lse,
+                                   const s2attn_plan *plan, const s2attn_shape *shape, void *stream)
+{
+    DArgs a = {};
+    const int rc = diff_args(a, k, v, q, lam, lam_dtype, quad_weights, plan, shape);
+    if (rc != S2ATTN_OK) return rc;
+    if (!y) return s2attn_fail(S2ATTN_E_INVALID, "null tensor pointer");
+    if (!y2 != !lse) return s2attn_fail(S2ATTN_E_INVALID, "y2 and lse are kept together or not at all");
+    if (lse && !aligned(lse, sizeof(float2))) return s2attn_fail(S2ATTN_E_INVALID, "lse must be 8-byte aligned");
+    a.y = y, a.y2 = y2, a.lse2 = reinterpret_cast<float2 *>(lse);
+    return launch_diff(FWD, a, shape->dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t s2attn_diff_backward_workspace_bytes(const s2attn_shape *shape)
+{
+    s2attn_shape sh;
+    const int rc = diff_shape(sh, shape);
+    if (rc != S2ATTN_OK) return rc;
+    return stat_points(&sh) * (int64_t)sizeof(float4) + round16(stat_points(&sh) * (int64_t)sizeof(float));
+}
+
+extern "C" int s2attn_diff_backward(const void *k, const void *v, const void *q, const void *lam, int lam_dtype, const void *dy, const void *y, const void *y2, const float *lse,
+                                    const float *quad_weights, void *dk, void *dv, void *dq, void *dlam, void *workspace, const s2attn_plan *plan, const s2attn_shape *shape, void *stream)
+{
+    DArgs a = {};
+    int rc = diff_args(a, k, v, q, lam, lam_dtype, quad_weights, plan, shape);
+    if (rc != S2ATTN_OK) return rc;
+    if (!dy || !y || !y2 || !lse || !dq || !workspace) return s2attn_fail(S2ATTN_E_INVALID, "null tensor pointer");
+    if (!dk != !dv) return s2attn_fail(S2ATTN_E_INVALID, "dk and dv are computed together or not at all");
+    if (!aligned(workspace, 16) || !aligned(lse, sizeof(float2))) return s2attn_fail(S2ATTN_E_INVALID, "workspace must be 16-byte and lse 8-byte aligned");
+    a.dy = dy, a.ysaved = y, a.y2saved = y2, a.lse2 = reinterpret_cast<float2 *>(const_cast<float *>(lse)), a.dq = dq, a.dk = dk, a.dv = dv, a.dlam = dlam;
+    a.dstats = static_cast<float4 *>(workspace);
+    a.lam_part = reinterpret_cast<float *>(a.dstats + stat_points(shape));
+    a.lam_n = shape->nlat_out * shape->nlon_out;
+    rc = launch_diff(DQ, a, shape->dtype, static_cast<hipStream_t>(stream));
+    if (rc != S2ATTN_OK || (!dk && !dlam)) return rc;
+    return launch_diff(DKDV, a, shape->dtype, static_cast<hipStream_t>(stream));
 }
 
 namespace {

@@ -783,6 +783,151 @@ Tensors13 layer_backward_op(const Tensor &grad, LAYER_ARGS, const Tensor &q, con
     return as_tuple(g);
 }
 
+// ---- differential attention -----------------------------------------------------------------------------------------------
+#define DIFF_ARGS                                                                                                                                              \
+    const Tensor &quad_weights, const Tensor &col_idx, const Tensor &row_off, int64_t num_heads, int64_t nlon_in, int64_t nlat_out, int64_t nlon_out
+#define DIFF_PLAN const c10::optional<Tensor> &plan, c10::OptionalArrayRef<int64_t> plan_header
+
+// t itself where the kernels read it in place (packed, or a column block of a wider buffer), else a packed copy
+Tensor in_place_or_packed(const Tensor &t)
+{
+    if (t.dim() != 4 || t.is_contiguous()) return t;
+    const int64_t ld = t.stride(2);
+    const bool block = t.stride(3) == 1 && ld >= t.size(3) && ld % 4 == 0 && t.stride(1) == t.size(2) * ld && t.stride(0) == t.size(1) * t.size(2) * ld && t.storage_offset() % 4 == 0;
+    return block ? t : t.contiguous();
+}
+
+void validate_diff(const Tensor &kx, const Tensor &vx, const Tensor &qy, const Tensor &lam, const Tensor *dy, DIFF_ARGS)
+{
+    TORCH_CHECK(qy.scalar_type() != at::kDouble, "differential attention takes fp32, bf16 and fp16 tensors, got ", qy.scalar_type());
+    TORCH_CHECK(num_heads < 1 || qy.dim() != 4 || qy.size(3) % (2 * num_heads) == 0, "q/k channel count (", qy.size(3), ") must be divisible by 2 * num_heads (", 2 * num_heads,
+                "): two maps per head");
+    TORCH_CHECK(num_heads < 1 || (lam.dim() == 1 && lam.size(0) == num_heads), "lam must hold one number per head (", num_heads, "), got a tensor of shape ", lam.sizes());
+    (void)dtype_code(lam.scalar_type());
+    validate(kx, vx, qy, dy, quad_weights, col_idx, row_off, num_heads, nlon_in, nlat_out, nlon_out);
+    require_gpu(lam, "lam", kx.device());
+}
+
+s2attn_shape diff_shape_of(const Tensor &kx, const Tensor &vx, const Tensor &qy, int64_t num_heads)
+{
+    s2attn_shape sh = shape_of(kx, vx, qy, num_heads);
+    sh.ck /= 2;
+    return sh;
+}
+
+// (y, y2, normalisers): the last two are what the backward needs, empty without `keep`
+std::tuple<Tensor, Tensor, Tensor> differential_forward(const Tensor &k_, const Tensor &v_, const Tensor &q_, const Tensor &lam_, DIFF_ARGS, bool keep, DIFF_PLAN)
+{
+    const Tensor kx = in_place_or_packed(k_), vx = in_place_or_packed(v_), qy = in_place_or_packed(q_);
+    validate_diff(kx, vx, qy, lam_, nullptr, quad_weights, col_idx, row_off, num_heads, nlon_in, nlat_out, nlon_out);
+    const Tensor lam = lam_.contiguous();
+    Tensor y = at::empty({kx.size(0), nlat_out, nlon_out, vx.size(3)}, kx.options());
+    Tensor y2 = keep ? at::empty_like(y) : at::empty({0}, kx.options());
+    Tensor lse = at::empty({0}, kx.options().dtype(at::kFloat));
+    if (keep) lse = at::empty({kx.size(0), num_heads, nlat_out * nlon_out, 2}, lse.options());
+    if (y.numel() == 0) return {y, y2, lse};
+    const s2attn_plan p = plan_for(col_idx, row_off, kx.size(1), nlon_in, nlat_out, nlon_out, plan, plan_header);
+    const s2attn_shape sh = diff_shape_of(kx, vx, qy, num_heads);
+    const Tensor qw = quad_weights.to(at::kFloat).contiguous();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(kx.device());
+    check_rc(s2attn_diff_forward(kx.data_ptr(), vx.data_ptr(), qy.data_ptr(), lam.data_ptr(), dtype_code(lam.scalar_type()), qw.data_ptr<float>(), y.data_ptr(),
+                                 keep ? y2.data_ptr() : nullptr, keep ? lse.data_ptr<float>() : nullptr, &p, &sh, current_stream(kx.device())),
+             "s2attn_diff_forward");
+    return {y, y2, lse};
+}
+
+// (dk, dv, dq, dlam); need: k or v, lam (what is not needed is returned empty; dq is a by-product of what the others need)
+std::tuple<Tensor, Tensor, Tensor, Tensor> differential_backward(const Tensor &dy_, const Tensor &k_, const Tensor &v_, const Tensor &q_, const Tensor &lam_, const Tensor &y,
+                                                                 const Tensor &y2, const Tensor &lse, DIFF_ARGS, std::array<bool, 2> need, DIFF_PLAN)
+{
+    const Tensor kx = in_place_or_packed(k_), vx = in_place_or_packed(v_), qy = in_place_or_packed(q_), dy = in_place_or_packed(dy_);
+    validate_diff(kx, vx, qy, lam_, &dy, quad_weights, col_idx, row_off, num_heads, nlon_in, nlat_out, nlon_out);
+    const Tensor lam = lam_.contiguous();
+    require_gpu(y, "y", kx.device()), require_gpu(y2, "y2", kx.device()), require_gpu(lse, "lse", kx.device());
+    TORCH_CHECK(y.sizes() == dy.sizes() && y.scalar_type() == dy.scalar_type() && y2.sizes() == dy.sizes() && y2.scalar_type() == dy.scalar_type() && y2.is_contiguous(),
+                "y and y2 must be the outputs of differential_forward with keep=True");
+    TORCH_CHECK(lse.dim() == 4 && lse.size(0) == kx.size(0) && lse.size(1) == num_heads && lse.size(2) == nlat_out * nlon_out && lse.size(3) == 2
+                    && lse.scalar_type() == at::kFloat && lse.is_contiguous(),
+                "lse must be the normalisers that differential_forward returned with keep=True");
+    const Tensor none = at::empty({0}, kx.options());
+    Tensor dq = at::empty(qy.sizes(), qy.options()), dk = need[0] ? at::empty(kx.sizes(), kx.options()) : none, dv = need[0] ? at::empty(vx.sizes(), vx.options()) : none;
+    Tensor dlam = need[1] ? at::empty(lam.sizes(), lam.options()) : none;
+    if (dy.numel() == 0) return {dk.zero_(), dv.zero_(), dq.zero_(), dlam.zero_()};
+    const s2attn_plan p = plan_for(col_idx, row_off, kx.size(1), nlon_in, nlat_out, nlon_out, plan, plan_header);
+    s2attn_shape sh = diff_shape_of(kx, vx, qy, num_heads);
+    sh.ld_dy = (int)point_stride(dy, "dy"), sh.ld_y = (int)point_stride(y, "y");
+    const int64_t nbytes = s2attn_diff_backward_workspace_bytes(&sh);
+    check_rc(nbytes, "s2attn_diff_backward_workspace_bytes");
+    Tensor ws = at::empty({nbytes / 4}, kx.options().dtype(at::kFloat));
+    const Tensor qw = quad_weights.to(at::kFloat).contiguous();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(kx.device());
+    check_rc(s2attn_diff_backward(kx.data_ptr(), vx.data_ptr(), qy.data_ptr(), lam.data_ptr(), dtype_code(lam.scalar_type()), dy.data_ptr(), y.data_ptr(), y2.data_ptr(),
+                                  lse.data_ptr<float>(), qw.data_ptr<float>(), need[0] ? dk.data_ptr() : nullptr, need[0] ? dv.data_ptr() : nullptr, dq.data_ptr(),
+                                  need[1] ? dlam.data_ptr() : nullptr, ws.data_ptr(), &p, &sh, current_stream(kx.device())),
+             "s2attn_diff_backward");
+    return {dk, dv, dq, dlam};
+}
+
+struct DiffState : torch::CustomClassHolder {
+    int64_t num_heads, nlon_in, nlat_out, nlon_out;
+    c10::optional<Tensor> plan;
+    std::vector<int64_t> plan_header;
+    c10::OptionalArrayRef<int64_t> header() const { return plan ? c10::OptionalArrayRef<int64_t>(plan_header) : c10::OptionalArrayRef<int64_t>(); }
+};
+
+struct DiffFunction : public torch::autograd::Function<DiffFunction> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &k, const Tensor &v, const Tensor &q, const Tensor &lam, const Tensor &quad_weights, const Tensor &col_idx,
+                          const Tensor &row_off, const c10::intrusive_ptr<DiffState> &s, bool keep)
+    {
+        auto [y, y2, lse] = differential_forward(k, v, q, lam, quad_weights, col_idx, row_off, s->num_heads, s->nlon_in, s->nlat_out, s->nlon_out, keep, s->plan, s->header());
+        if (keep) {
+            ctx->save_for_backward({k, v, q, lam, y, y2, lse, quad_weights, col_idx, row_off});
+            ctx->saved_data["state"] = c10::IValue::make_capsule(s);
+            ctx->set_materialize_grads(false);
+        }
+        return y;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        torch::autograd::variable_list r(9);
+        if (!grads[0].defined()) return r;
+        const auto held = ctx->saved_data["state"].toCapsule();
+        const DiffState &s = *static_cast<const DiffState *>(held.get());
+        const auto t = ctx->get_saved_variables();
+        const std::array<bool, 2> need = {ctx->needs_input_grad(0) || ctx->needs_input_grad(1), ctx->needs_input_grad(3)};
+        std::tuple<Tensor, Tensor, Tensor, Tensor> g;
+        // (create_graph=True: the operator ties the gradients to what they depend on, and refuses to be differentiated)
+        if (observed(grads[0]) || c10::GradMode::is_enabled()) {
+            static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("s2attn_kernels::differential_backward", "").typed<decltype(differential_backward)>();
+            g = op.call(grads[0], t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], s.num_heads, s.nlon_in, s.nlat_out, s.nlon_out, need, s.plan, s.header());
+        } else {
+            g = differential_backward(grads[0], t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], s.num_heads, s.nlon_in, s.nlat_out, s.nlon_out, need, s.plan, s.header());
+        }
+        if (ctx->needs_input_grad(0)) r[0] = std::get<0>(g);
+        if (ctx->needs_input_grad(1)) r[1] = std::get<1>(g);
+        if (ctx->needs_input_grad(2)) r[2] = std::get<2>(g);
+        if (ctx->needs_input_grad(3)) r[3] = std::get<3>(g);
+        return r;
+    }
+};
+
+// eager mode: one C++ autograd node
+Tensor differential_attention(const Tensor &k, const Tensor &v, const Tensor &q, const Tensor &lam, DIFF_ARGS, DIFF_PLAN)
+{
+    const Tensor t[] = {k, v, q, lam, quad_weights, col_idx, row_off};
+    const bool keep = c10::GradMode::is_enabled() && (k.requires_grad() || v.requires_grad() || q.requires_grad() || lam.requires_grad());
+    if (c10::impl::dispatch_mode_enabled() || at::areAnyTensorSubclassLike(t)) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("s2attn_kernels::differential_forward", "").typed<decltype(differential_forward)>();
+        return std::get<0>(op.call(k, v, q, lam, quad_weights, col_idx, row_off, num_heads, nlon_in, nlat_out, nlon_out, keep, plan, plan_header));
+    }
+    auto s = c10::make_intrusive<DiffState>();
+    s->num_heads = num_heads, s->nlon_in = nlon_in, s->nlat_out = nlat_out, s->nlon_out = nlon_out;
+    if (plan && plan_header) s->plan = plan, s->plan_header = plan_header->vec();
+    // (a copy belongs to the graph, so it is made ahead of the node)
+    return DiffFunction::apply(in_place_or_packed(k), in_place_or_packed(v), in_place_or_packed(q), lam, quad_weights, col_idx, row_off, s, keep);
+}
+
 // ---- layout ---------------------------------------------------------------------------------------------------------------
 Tensor permute(const Tensor &x, bool to_nhwc)
 {
@@ -856,6 +1001,13 @@ TORCH_LIBRARY(s2attn_kernels, m)
     std::string thirteen = "Tensor";
     for (int i = 1; i < NGRADS; i++) thirteen += ", Tensor";
     m.def(("layer_backward(Tensor grad, " + layer + ", Tensor q, Tensor k, Tensor v, Tensor q_raw, Tensor k_raw, Tensor y, Tensor lse, bool[13] need) -> (" + thirteen + ")").c_str(), {at::Tag::pt2_compliant_tag});
+    // differential attention: the composite operator makes its autograd node inside; its two steps are what a traced graph records
+    const std::string tensors = "Tensor kx, Tensor vx, Tensor qy, Tensor lam", rest = "Tensor quad_weights, Tensor col_idx, Tensor row_off, int num_heads, int nlon_in, int nlat_out, int nlon_out",
+                      plan = "Tensor? plan=None, int[]? plan_header=None";
+    m.def(("differential_attention(" + tensors + ", " + rest + ", " + plan + ") -> Tensor").c_str(), &differential_attention);
+    m.def(("differential_forward(" + tensors + ", " + rest + ", bool keep, " + plan + ") -> (Tensor, Tensor, Tensor)").c_str(), {at::Tag::pt2_compliant_tag});
+    m.def(("differential_backward(Tensor dy, " + tensors + ", Tensor y, Tensor y2, Tensor lse, " + rest + ", bool[2] need, " + plan + ") -> (Tensor, Tensor, Tensor, Tensor)").c_str(),
+          {at::Tag::pt2_compliant_tag});
 }
 
 TORCH_LIBRARY_IMPL(s2attn_kernels, CUDA, m)
@@ -864,6 +1016,8 @@ TORCH_LIBRARY_IMPL(s2attn_kernels, CUDA, m)
     m.impl("backward_saved", &backward_saved);
     m.impl("layer_forward", &layer_forward_op);
     m.impl("layer_backward", &layer_backward_op);
+    m.impl("differential_forward", &differential_forward);
+    m.impl("differential_backward", &differential_backward);
 }
 
 TORCH_LIBRARY_IMPL(s2attn_kernels, CPU, m) // fails with the same message as above
@@ -872,4 +1026,6 @@ TORCH_LIBRARY_IMPL(s2attn_kernels, CPU, m) // fails with the same message as abo
     m.impl("backward_saved", &backward_saved);
     m.impl("layer_forward", &layer_forward_op);
     m.impl("layer_backward", &layer_backward_op);
+    m.impl("differential_forward", &differential_forward);
+    m.impl("differential_backward", &differential_backward);
 }

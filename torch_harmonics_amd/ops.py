@@ -350,6 +350,71 @@ def _(grad, *args, out_shape=None, **kwargs) -> int:
     return 2 * (sum(n for n, wanted in zip((q, k, v), to_input) if wanted) + sum(n for n, wanted in zip((q, k, v, p), need[3:7]) if wanted) + (p if through else 0))
 
 
+# ---- differential attention ---------------------------------------------------------------------------------------------------
+# s2attn_kernels::differential_attention is one C++ autograd node in eager mode; its two steps are operators for traced graphs.
+differential_forward = torch.ops.s2attn_kernels.differential_forward.default
+differential_backward = torch.ops.s2attn_kernels.differential_backward.default
+
+
+@torch.library.register_fake("s2attn_kernels::differential_forward")
+def _(kx, vx, qy, lam, quad_weights, col_idx, row_off, num_heads, nlon_in, nlat_out, nlon_out, keep, plan=None, plan_header=None):
+    y = kx.new_empty((kx.shape[0], nlat_out, nlon_out, vx.shape[3]))
+    if not keep:
+        return y, kx.new_empty((0,)), kx.new_empty((0,), dtype=torch.float32)
+    return y, torch.empty_like(y), kx.new_empty((kx.shape[0], num_heads, nlat_out * nlon_out, 2), dtype=torch.float32)
+
+
+@torch.library.register_fake("s2attn_kernels::differential_backward")
+def _(dy, kx, vx, qy, lam, y, y2, lse, quad_weights, col_idx, row_off, num_heads, nlon_in, nlat_out, nlon_out, need, plan=None, plan_header=None):
+    none = lambda: kx.new_empty((0,))  # noqa: E731
+    packed = lambda t, wanted=True: t.new_empty(t.shape) if wanted else none()  # noqa: E731
+    return packed(kx, need[0]), packed(vx, need[0]), packed(qy), packed(lam, need[1])
+
+
+def _differential_setup_context(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:7], *output)
+    ctx.heads_and_grids, ctx.keep, ctx.plan, ctx.ninputs = inputs[7:11], inputs[11], (inputs[12:] + (None, None))[:2], len(inputs)
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.set_materialize_grads(False)
+
+
+def _differential_backward_rule(ctx, grad, *rest):
+    if grad is None:
+        return (None,) * ctx.ninputs
+    if not ctx.keep:
+        raise RuntimeError("differential_forward ran with keep=False: nothing of it is left for a backward")
+    kx, vx, qy, lam, quad_weights, col_idx, row_off, y, y2, lse = ctx.saved_tensors
+    wanted = ctx.needs_input_grad
+    grads = differential_backward(grad, kx, vx, qy, lam, y, y2, lse, quad_weights, col_idx, row_off, *ctx.heads_and_grids, [wanted[0] or wanted[1], wanted[3]], *ctx.plan)
+    return (*[g if w else None for g, w in zip(grads, wanted)], *(None,) * (ctx.ninputs - 4))
+
+
+def _no_second_derivative_of_differential(ctx, *grads):
+    raise RuntimeError("the gradients of differential attention cannot be differentiated")
+
+
+torch.library.register_autograd("s2attn_kernels::differential_backward", _no_second_derivative_of_differential, setup_context=_no_context)
+torch.library.register_autograd("s2attn_kernels::differential_forward", _differential_backward_rule, setup_context=_differential_setup_context)
+
+
+def differential_s2_attention(kw, vw, qw, lam, quad_weights, col_idx, row_off, nh, nlon_in, nlat_out, nlon_out, plan=None, plan_header=None):
+    """Differentiable differential attention on NHWC heads-packed tensors: the difference of two softmax maps over each point's neighborhood,
+    y = sum_j (p1_j - lam p2_j) v_j with p1, p2 the quadrature-weighted softmaxes of q1.k1 and q2.k2.
+
+    qw (B, nlat_out, nlon_out, nh * 2 * ck) and kw (B, nlat_in, nlon_in, nh * 2 * ck) hold two vectors per head, (q1 | q2) of head 0 first, the
+    softmax scale already on the query; vw (B, nlat_in, nlon_in, nh * cv); lam (nh,), fp32 or 16-bit, any sign.  The other arguments are
+    those of neighborhood_s2_attention, in all three directions.  Tensors are fp32, bf16 or fp16 (sums in fp32); packed ones and column
+    blocks of a wider buffer are read in place, others are copied.  Under autocast k, v and q are brought to its type.  A point that sees
+    nothing has y = 0.  Gradients of all four, the same in every run; they cannot be differentiated again."""
+    if torch.is_autocast_enabled(qw.device.type):
+        dtype = torch.get_autocast_dtype(qw.device.type)
+        kw, vw, qw = kw.to(dtype), vw.to(dtype), qw.to(dtype)
+    if torch.compiler.is_compiling():
+        keep = torch.is_grad_enabled() and any(t.requires_grad for t in (kw, vw, qw, lam))
+        return differential_forward(kw, vw, qw, lam, quad_weights, col_idx, row_off, nh, nlon_in, nlat_out, nlon_out, keep, plan, plan_header)[0]
+    return torch.ops.s2attn_kernels.differential_attention.default(kw, vw, qw, lam, quad_weights, col_idx, row_off, nh, nlon_in, nlat_out, nlon_out, plan, plan_header)
+
+
 # Autocast: k, v, q are brought to the active autocast dtype and the op re-entered with autocast off;
 # quad_weights and the index tensors pass through (attention_optimized.py:310-322).
 def _make_autocast_impl(device_type: str):
