@@ -294,6 +294,38 @@ int s2attn_diff_backward(const void *k, const void *v, const void *q, const void
                          const float *quad_weights, void *dk, void *dv, void *dq, void *dlam, void *workspace, const s2attn_plan *plan, const s2attn_shape *shape, void *stream);
 
 /*
+ * Group norm with an activation on channels-last tensors [batch, nlat, nlon, channels]: y = act((x - mean) / sqrt(var + eps) weight + bias), mean
+ * and (biased) variance over the grid and the channels of a group; with ring_weights (fp32 [nlat], not negative) every point counts by its
+ * ring's, and a ring of weight zero is not looked at for the statistics (weights that are zero everywhere: mean and variance zero).  It has
+ * no counterpart in the reference.  Any channel counts; x and dy may be column blocks (ld_x, ld_dy: elements between two points, 0 =
+ * packed).  weight and bias: param_dtype, may be null (1 and 0).  Sums in fp32 (over workgroups in 64 bits or as moments), the same in
+ * every run; no atomics.  stats [batch][groups][3] fp32 (mean, 1 / sqrt(var + eps), 1 / sum of weights): written by the forward, read by the
+ * backward, which writes dx, dweight and dbias (any of them may be null).  workspace: s2attn_group_norm_workspace_bytes(n, backward) of
+ * device memory, 8-byte aligned; calls that overlap need one each.
+ */
+#define S2ATTN_ACT_NONE 0
+#define S2ATTN_ACT_RELU 1
+#define S2ATTN_ACT_SILU 2
+#define S2ATTN_ACT_GELU 3 /* with the error function */
+typedef struct s2attn_gnorm {
+    int batch, nlat, nlon, channels, groups;
+    int dtype, param_dtype, activation;
+    int ld_x, ld_dy;
+    float eps;
+    const void *x, *weight, *bias;
+    const float *ring_weights;
+    void *y;
+    float *stats;
+    const void *dy;
+    void *dx, *dweight, *dbias;
+    void *workspace;
+} s2attn_gnorm;
+
+int64_t s2attn_group_norm_workspace_bytes(const s2attn_gnorm *n, int backward);
+int s2attn_group_norm(const s2attn_gnorm *n, void *stream);
+int s2attn_group_norm_backward(const s2attn_gnorm *n, void *stream);
+
+/*
  * Layout conversion.  Replace attention_kernels::permute_to_nhwc / permute_to_nchw
  * (attention_interface.cpp:85-86; CUDA kernels attention_cuda_utils.cuh:417-576).
  * Pure element moves; elem_size is 2, 4 or 8 bytes.  dst must not alias src.

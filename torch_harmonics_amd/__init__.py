@@ -8,7 +8,7 @@ from . import _lib
 from ._layout import to_nchw, to_nhwc
 from .attention import NeighborhoodAttentionS2
 from .neighborhood import precompute_neighborhood_s2
-from .ops import _neighborhood_s2_attention_optimized, differential_s2_attention, neighborhood_s2_attention
+from .ops import _neighborhood_s2_attention_optimized, differential_s2_attention, group_norm_s2, neighborhood_s2_attention
 from .quadrature import precompute_latitudes, precompute_longitudes
 
 __all__ = [
@@ -16,6 +16,7 @@ __all__ = [
     "_neighborhood_s2_attention_optimized",
     "neighborhood_s2_attention",
     "differential_s2_attention",
+    "group_norm_s2",
     "to_nhwc",
     "to_nchw",
     "precompute_neighborhood_s2",

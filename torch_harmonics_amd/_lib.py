@@ -97,6 +97,16 @@ class NormStruct(ctypes.Structure):
     ]  # fmt: skip
 
 
+class GroupNormStruct(ctypes.Structure):
+    _fields_ = [(n, _int) for n in ("batch", "nlat", "nlon", "channels", "groups", "dtype", "param_dtype", "activation", "ld_x", "ld_dy")] + [("eps", ctypes.c_float)] + [
+        (n, _vp) for n in ("x", "weight", "bias", "ring_weights", "y", "stats", "dy", "dx", "dweight", "dbias", "workspace")
+    ]  # fmt: skip
+
+
+# activations of the group norm, by their codes in include/s2attn.h
+ACTIVATIONS = ("none", "relu", "silu", "gelu")
+
+
 class RingShapeStruct(ctypes.Structure):
     _fields_ = [
         ("batch", ctypes.c_int32),
@@ -145,6 +155,9 @@ SYMBOLS = {
     "s2attn_diff_forward": (_int, [_vp] * 4 + [_int] + [_vp] * 4 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
     "s2attn_diff_backward_workspace_bytes": (_i64, [ctypes.POINTER(ShapeStruct)]),
     "s2attn_diff_backward": (_int, [_vp] * 4 + [_int] + [_vp] * 10 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
+    "s2attn_group_norm_workspace_bytes": (_i64, [ctypes.POINTER(GroupNormStruct), _int]),
+    "s2attn_group_norm": (_int, [ctypes.POINTER(GroupNormStruct), _vp]),
+    "s2attn_group_norm_backward": (_int, [ctypes.POINTER(GroupNormStruct), _vp]),
     "s2attn_permute_to_nhwc": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _int, _vp]),
     "s2attn_permute_to_nchw": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _int, _vp]),
     "s2attn_pack_k16": (_int, [_int, _int]),

@@ -928,6 +928,134 @@ Tensor differential_attention(const Tensor &k, const Tensor &v, const Tensor &q,
     return DiffFunction::apply(in_place_or_packed(k), in_place_or_packed(v), in_place_or_packed(q), lam, quad_weights, col_idx, row_off, s, keep);
 }
 
+// ---- group norm --------------------------------------------------------------------------------------------------------------
+using MaybeTensor = c10::optional<Tensor>;
+Tensor or_none(const MaybeTensor &t) { return t.has_value() ? *t : Tensor(); }
+
+s2attn_gnorm gnorm_args(const Tensor &x, int64_t groups, const Tensor &weight, const Tensor &bias, const Tensor &quad, double eps, int64_t activation)
+{
+    TORCH_CHECK(x.dim() == 4, "x must be a 4-dimensional (B, nlat, nlon, channels) tensor, got ", x.dim(), " dimensions");
+    TORCH_CHECK(groups >= 1 && x.size(3) % groups == 0, groups, " groups do not divide ", x.size(3), " channels");
+    TORCH_CHECK(eps >= 0, "eps must not be negative, got ", eps);
+    s2attn_gnorm n = {};
+    n.dtype = dtype_code(x.scalar_type()), n.param_dtype = S2ATTN_F32;
+    for (const Tensor *p : {&weight, &bias}) {
+        if (!p->defined()) continue;
+        TORCH_CHECK(p->dim() == 1 && p->size(0) == x.size(3), "weight and bias must hold one number per channel (", x.size(3), "), got a tensor of shape ", p->sizes());
+        TORCH_CHECK(!weight.defined() || p->scalar_type() == weight.scalar_type(), "weight and bias must share a dtype");
+        n.param_dtype = dtype_code(p->scalar_type());
+    }
+    TORCH_CHECK(!quad.defined() || quad.numel() == x.size(1), "quad_weights must have nlat = ", x.size(1), " entries, got ", quad.defined() ? quad.numel() : 0);
+    TORCH_CHECK(x.numel() == 0 || (x.size(0) < (int64_t)1 << 31 && x.size(1) < (int64_t)1 << 31 && x.size(2) < (int64_t)1 << 31 && x.size(3) < (int64_t)1 << 31), "extents must be below 2^31");
+    require_gpu(x, "x", x.device());
+    if (weight.defined()) require_gpu(weight, "weight", x.device());
+    if (bias.defined()) require_gpu(bias, "bias", x.device());
+    if (quad.defined()) require_gpu(quad, "quad_weights", x.device());
+    n.batch = (int)x.size(0), n.nlat = (int)x.size(1), n.nlon = (int)x.size(2), n.channels = (int)x.size(3), n.groups = (int)groups;
+    n.activation = (int)activation, n.eps = (float)eps;
+    return n;
+}
+const void *ptr_or_null(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// (y, statistics)
+std::tuple<Tensor, Tensor> group_norm_forward(const Tensor &x_, int64_t groups, const MaybeTensor &weight_, const MaybeTensor &bias_, const MaybeTensor &quad_, double eps, int64_t activation)
+{
+    const Tensor x = in_place_or_packed(x_);
+    Tensor weight = or_none(weight_), bias = or_none(bias_), quad = or_none(quad_);
+    s2attn_gnorm n = gnorm_args(x, groups, weight, bias, quad, eps, activation);
+    weight = dense(weight), bias = dense(bias);
+    if (quad.defined()) quad = quad.to(at::kFloat).contiguous();
+    Tensor y = at::empty(x.sizes(), x.options()), stats = at::empty({x.size(0), groups, 3}, x.options().dtype(at::kFloat));
+    if (x.numel() == 0) return {y, stats.zero_()};
+    n.ld_x = (int)point_stride(x, "x");
+    const int64_t bytes = s2attn_group_norm_workspace_bytes(&n, 0);
+    check_rc(bytes, "s2attn_group_norm");
+    const Tensor ws = at::empty({(bytes + 7) / 8}, x.options().dtype(at::kDouble));
+    n.x = x.data_ptr(), n.weight = ptr_or_null(weight), n.bias = ptr_or_null(bias), n.ring_weights = static_cast<const float *>(ptr_or_null(quad));
+    n.y = y.data_ptr(), n.stats = stats.data_ptr<float>(), n.workspace = ws.data_ptr();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    check_rc(s2attn_group_norm(&n, current_stream(x.device())), "s2attn_group_norm");
+    return {y, stats};
+}
+
+// (dx, dweight, dbias); what is not needed is returned empty
+std::tuple<Tensor, Tensor, Tensor> group_norm_backward(const Tensor &dy_, const Tensor &x_, int64_t groups, const MaybeTensor &weight_, const MaybeTensor &bias_, const MaybeTensor &quad_,
+                                                       const Tensor &stats, double eps, int64_t activation, std::array<bool, 3> need)
+{
+    const Tensor x = in_place_or_packed(x_), dy = in_place_or_packed(dy_);
+    Tensor weight = or_none(weight_), bias = or_none(bias_), quad = or_none(quad_);
+    s2attn_gnorm n = gnorm_args(x, groups, weight, bias, quad, eps, activation);
+    TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(), "dy must have the shape and dtype of x");
+    require_gpu(dy, "dy", x.device()), require_gpu(stats, "statistics", x.device());
+    TORCH_CHECK(stats.dim() == 3 && stats.size(0) == x.size(0) && stats.size(1) == groups && stats.size(2) == 3 && stats.scalar_type() == at::kFloat && stats.is_contiguous(),
+                "statistics must be those that group_norm_forward returned");
+    weight = dense(weight), bias = dense(bias);
+    if (quad.defined()) quad = quad.to(at::kFloat).contiguous();
+    const Tensor none = at::empty({0}, x.options());
+    need[1] = need[1] && weight.defined(), need[2] = need[2] && bias.defined();
+    Tensor dx = need[0] ? at::empty(x.sizes(), x.options()) : none, dw = need[1] ? at::empty(weight.sizes(), weight.options()) : none, db = need[2] ? at::empty(bias.sizes(), bias.options()) : none;
+    if (x.numel() == 0) return {dx, dw.zero_(), db.zero_()};
+    n.ld_x = (int)point_stride(x, "x"), n.ld_dy = (int)point_stride(dy, "dy");
+    const int64_t bytes = s2attn_group_norm_workspace_bytes(&n, 1);
+    check_rc(bytes, "s2attn_group_norm_backward");
+    const Tensor ws = at::empty({(bytes + 7) / 8}, x.options().dtype(at::kDouble));
+    n.x = x.data_ptr(), n.dy = dy.data_ptr(), n.weight = ptr_or_null(weight), n.bias = ptr_or_null(bias), n.ring_weights = static_cast<const float *>(ptr_or_null(quad));
+    n.stats = stats.data_ptr<float>(), n.workspace = ws.data_ptr();
+    n.dx = need[0] ? dx.data_ptr() : nullptr, n.dweight = need[1] ? dw.data_ptr() : nullptr, n.dbias = need[2] ? db.data_ptr() : nullptr;
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    check_rc(s2attn_group_norm_backward(&n, current_stream(x.device())), "s2attn_group_norm_backward");
+    return {dx, dw, db};
+}
+
+struct GroupNormFunction : public torch::autograd::Function<GroupNormFunction> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias, const MaybeTensor &quad, int64_t groups, double eps, int64_t activation,
+                          bool keep)
+    {
+        auto [y, stats] = group_norm_forward(x, groups, weight, bias, quad, eps, activation);
+        if (keep) {
+            ctx->save_for_backward({x, or_none(weight), or_none(bias), or_none(quad), stats});
+            ctx->saved_data["groups"] = groups, ctx->saved_data["eps"] = eps, ctx->saved_data["activation"] = activation;
+            ctx->set_materialize_grads(false);
+        }
+        return y;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        torch::autograd::variable_list r(8);
+        if (!grads[0].defined()) return r;
+        const auto t = ctx->get_saved_variables();
+        const int64_t groups = ctx->saved_data["groups"].toInt(), activation = ctx->saved_data["activation"].toInt();
+        const double eps = ctx->saved_data["eps"].toDouble();
+        const bool w = t[1].defined(), bias = t[2].defined(); // (an absent tensor has no place among the node's inputs)
+        const std::array<bool, 3> need = {ctx->needs_input_grad(0), w && ctx->needs_input_grad(1), bias && ctx->needs_input_grad(w ? 2 : 1)};
+        std::tuple<Tensor, Tensor, Tensor> g;
+        if (observed(grads[0]) || c10::GradMode::is_enabled()) {
+            static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("s2attn_kernels::group_norm_backward", "").typed<decltype(group_norm_backward)>();
+            g = op.call(grads[0], t[0], groups, given_or_none(t[1]), given_or_none(t[2]), given_or_none(t[3]), t[4], eps, activation, need);
+        } else {
+            g = group_norm_backward(grads[0], t[0], groups, given_or_none(t[1]), given_or_none(t[2]), given_or_none(t[3]), t[4], eps, activation, need);
+        }
+        if (need[0]) r[0] = std::get<0>(g);
+        if (need[1]) r[1] = std::get<1>(g);
+        if (need[2]) r[2] = std::get<2>(g);
+        return r;
+    }
+};
+
+// eager mode: one C++ autograd node
+Tensor group_norm(const Tensor &x, int64_t groups, const MaybeTensor &weight, const MaybeTensor &bias, const MaybeTensor &quad, double eps, int64_t activation)
+{
+    const Tensor t[] = {x, or_none(weight), or_none(bias), or_none(quad)};
+    bool any = false;
+    for (const Tensor &p : t) any |= p.defined() && p.requires_grad();
+    if (c10::impl::dispatch_mode_enabled() || at::areAnyTensorSubclassLike(t)) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("s2attn_kernels::group_norm_forward", "").typed<decltype(group_norm_forward)>();
+        return std::get<0>(op.call(x, groups, weight, bias, quad, eps, activation));
+    }
+    return GroupNormFunction::apply(in_place_or_packed(x), weight, bias, quad, groups, eps, activation, any && c10::GradMode::is_enabled());
+}
+
 // ---- layout ---------------------------------------------------------------------------------------------------------------
 Tensor permute(const Tensor &x, bool to_nhwc)
 {
@@ -1004,6 +1132,10 @@ TORCH_LIBRARY(s2attn_kernels, m)
     // differential attention: the composite operator makes its autograd node inside; its two steps are what a traced graph records
     const std::string tensors = "Tensor kx, Tensor vx, Tensor qy, Tensor lam", rest = "Tensor quad_weights, Tensor col_idx, Tensor row_off, int num_heads, int nlon_in, int nlat_out, int nlon_out",
                       plan = "Tensor? plan=None, int[]? plan_header=None";
+    const std::string norm = "int groups, Tensor? weight, Tensor? bias, Tensor? quad_weights, ";
+    m.def(("group_norm(Tensor x, " + norm + "float eps, int activation) -> Tensor").c_str(), &group_norm);
+    m.def(("group_norm_forward(Tensor x, " + norm + "float eps, int activation) -> (Tensor, Tensor)").c_str(), {at::Tag::pt2_compliant_tag});
+    m.def(("group_norm_backward(Tensor dy, Tensor x, " + norm + "Tensor stats, float eps, int activation, bool[3] need) -> (Tensor, Tensor, Tensor)").c_str(), {at::Tag::pt2_compliant_tag});
     m.def(("differential_attention(" + tensors + ", " + rest + ", " + plan + ") -> Tensor").c_str(), &differential_attention);
     m.def(("differential_forward(" + tensors + ", " + rest + ", bool keep, " + plan + ") -> (Tensor, Tensor, Tensor)").c_str(), {at::Tag::pt2_compliant_tag});
     m.def(("differential_backward(Tensor dy, " + tensors + ", Tensor y, Tensor y2, Tensor lse, " + rest + ", bool[2] need, " + plan + ") -> (Tensor, Tensor, Tensor, Tensor)").c_str(),
@@ -1018,6 +1150,8 @@ TORCH_LIBRARY_IMPL(s2attn_kernels, CUDA, m)
     m.impl("layer_backward", &layer_backward_op);
     m.impl("differential_forward", &differential_forward);
     m.impl("differential_backward", &differential_backward);
+    m.impl("group_norm_forward", &group_norm_forward);
+    m.impl("group_norm_backward", &group_norm_backward);
 }
 
 TORCH_LIBRARY_IMPL(s2attn_kernels, CPU, m) // fails with the same message as above
@@ -1028,4 +1162,6 @@ TORCH_LIBRARY_IMPL(s2attn_kernels, CPU, m) // fails with the same message as abo
     m.impl("layer_backward", &layer_backward_op);
     m.impl("differential_forward", &differential_forward);
     m.impl("differential_backward", &differential_backward);
+    m.impl("group_norm_forward", &group_norm_forward);
+    m.impl("group_norm_backward", &group_norm_backward);
 }

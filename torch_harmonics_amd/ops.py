@@ -415,6 +415,66 @@ def differential_s2_attention(kw, vw, qw, lam, quad_weights, col_idx, row_off, n
     return torch.ops.s2attn_kernels.differential_attention.default(kw, vw, qw, lam, quad_weights, col_idx, row_off, nh, nlon_in, nlat_out, nlon_out, plan, plan_header)
 
 
+# ---- group norm ---------------------------------------------------------------------------------------------------------------
+# s2attn_kernels::group_norm is one C++ autograd node in eager mode; its two steps are operators for traced graphs.
+group_norm_forward = torch.ops.s2attn_kernels.group_norm_forward.default
+group_norm_backward = torch.ops.s2attn_kernels.group_norm_backward.default
+
+
+@torch.library.register_fake("s2attn_kernels::group_norm_forward")
+def _(x, groups, weight, bias, quad_weights, eps, activation):
+    return x.new_empty(x.shape), x.new_empty((x.shape[0], groups, 3), dtype=torch.float32)
+
+
+@torch.library.register_fake("s2attn_kernels::group_norm_backward")
+def _(dy, x, groups, weight, bias, quad_weights, stats, eps, activation, need):
+    return tuple(t.new_empty(t.shape) if n and t is not None else x.new_empty((0,)) for t, n in zip((x, weight, bias), need))
+
+
+def _group_norm_setup_context(ctx, inputs, output):
+    x, groups, weight, bias, quad_weights, eps, activation = inputs
+    ctx.save_for_backward(x, weight, bias, quad_weights, output[1])
+    ctx.options = groups, eps, activation
+    ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
+
+
+def _group_norm_backward_rule(ctx, grad, grad_stats):
+    if grad is None:
+        return (None,) * 7
+    x, weight, bias, quad_weights, stats = ctx.saved_tensors
+    groups, eps, activation = ctx.options
+    wanted = ctx.needs_input_grad
+    need = [wanted[0], wanted[2], wanted[3]]
+    dx, dw, db = [g if n else None for g, n in zip(group_norm_backward(grad, x, groups, weight, bias, quad_weights, stats, eps, activation, need), need)]
+    return dx, None, dw, db, None, None, None
+
+
+def _no_second_derivative_of_norm(ctx, *grads):
+    raise RuntimeError("the gradients of the group norm cannot be differentiated")
+
+
+torch.library.register_autograd("s2attn_kernels::group_norm_backward", _no_second_derivative_of_norm, setup_context=_no_context)
+torch.library.register_autograd("s2attn_kernels::group_norm_forward", _group_norm_backward_rule, setup_context=_group_norm_setup_context)
+
+
+def group_norm_s2(x, num_groups, weight=None, bias=None, quad_weights=None, eps=1e-5, activation=None):
+    """Differentiable group norm with an activation on NHWC tensors: y = act((x - mean) / sqrt(var + eps) * weight + bias), mean and biased variance
+    over the grid and the channels of a group.
+
+    x (B, nlat, nlon, C), fp32, bf16 or fp16 (statistics in fp32), packed or a column block of a wider buffer (others are copied); weight, bias
+    (C,) of one type, or None; quad_weights (nlat,): every point counts by its latitude ring's weight (the grid's quadrature: statistics
+    by area), not negative, no gradient; a ring of weight zero is not looked at for the statistics.  activation: None (or "none"), "relu",
+    "silu", "gelu" (with the error function).  Gradients of x, weight and bias, the same in every run; they cannot be differentiated again."""
+    name = "none" if activation is None else activation
+    if name not in _lib.ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}: one of {', '.join(_lib.ACTIVATIONS)}, or None")
+    code = _lib.ACTIVATIONS.index(name)
+    if torch.compiler.is_compiling():
+        return group_norm_forward(x, num_groups, weight, bias, quad_weights, eps, code)[0]
+    return torch.ops.s2attn_kernels.group_norm.default(x, num_groups, weight, bias, quad_weights, eps, code)
+
+
 # Autocast: k, v, q are brought to the active autocast dtype and the op re-entered with autocast off;
 # quad_weights and the index tensors pass through (attention_optimized.py:310-322).
 def _make_autocast_impl(device_type: str):
