@@ -101,3 +101,31 @@ def test_entry_points_refuse_bad_arguments_before_touching_the_gpu():
     says(backward(y2=None), -1, "null tensor")
     says(lib.s2attn_diff_backward_workspace_bytes(ctypes.byref(shape(ck=300))), -2, "1 to 256")
     assert lib.s2attn_diff_backward_workspace_bytes(ctypes.byref(shape())) == 2 * 72 * 20
+
+
+def test_module_state_and_refusals():
+    m = th.DifferentialNeighborhoodAttentionS2(16, (8, 16), (8, 16), num_heads=2, use_qknorm=True)
+    assert m.scale == 1 / 2 and m.q_norm_weights.shape == (4,) and m.lambda_q1.shape == (2, 4) and m.learned_lambda().shape == (2,)
+    base = th.NeighborhoodAttentionS2(16, (8, 16), (8, 16), num_heads=2)
+    assert set(base.state_dict()) <= set(m.state_dict())
+    assert set(m.state_dict()) - set(base.state_dict()) == {"lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2", "q_norm_weights", "k_norm_weights", "head_norm.weight", "head_norm.bias"}
+    with pytest.raises(ValueError, match="two maps per head"):
+        th.DifferentialNeighborhoodAttentionS2(12, (8, 16), (8, 16), num_heads=4)
+    with pytest.raises(ValueError, match="unknown norm"):
+        th.DifferentialNeighborhoodAttentionS2(16, (8, 16), (8, 16), norm="layer")
+    with pytest.raises(ValueError, match="part of the group norm"):
+        th.DifferentialNeighborhoodAttentionS2(16, (8, 16), (8, 16), norm="rms", activation="silu")
+    with pytest.raises(RuntimeError, match="only run on a ROCm GPU"):
+        m(torch.zeros(1, 16, 8, 16))
+    with pytest.raises(RuntimeError, match="query latitudes"):
+        m(torch.zeros(1, 16, 9, 16))
+    with pytest.raises(ValueError, match="divides num_channels"):
+        th.GroupNormS2(3, 16)
+    with pytest.raises(ValueError, match="unknown activation"):
+        th.GroupNormS2(4, 16, activation="tanh")
+    n = th.GroupNormS2(4, 16, (8, 16))
+    assert abs(n.quad_weights.sum().item() * 16 - 12.566371) < 1e-4 and set(n.state_dict()) == {"weight", "bias"}
+    with pytest.raises(RuntimeError, match="input longitudes"):
+        n(torch.zeros(1, 16, 8, 15))
+    with pytest.raises(RuntimeError, match="input channels"):
+        n(torch.zeros(1, 15, 8, 16))

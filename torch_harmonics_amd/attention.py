@@ -560,6 +560,10 @@ class NeighborhoodAttentionS2(nn.Module):
             self.psi_plan, self._psi_plan_header,
         )  # fmt: skip
 
+        return self._project(out, direct)
+
+    def _project(self, out: torch.Tensor, direct: bool) -> torch.Tensor:
+        """The output projection, NHWC -> NCHW."""
         wp = self.proj_weights.view(self.proj_weights.shape[0], -1)
         if direct and out.dtype == torch.float32 and out.is_contiguous():
             return _Linear1x1ToNCHW.apply(out, wp, self.proj_bias)
