@@ -288,6 +288,10 @@ int s2attn_backward_saved_noalloc(const void *k, const void *v, const void *q, c
 int s2attn_diff_forward(const void *k, const void *v, const void *q, const void *lam, int lam_dtype, const float *quad_weights, void *y, void *y2, float *lse,
                         const s2attn_plan *plan, const s2attn_shape *shape, void *stream);
 
+/* The family of kernels (S2ATTN_FAMILY_...) that a call of this problem runs on when every tensor's address is a multiple of `alignment`
+ * bytes, or a negative error.  Host only. */
+int s2attn_diff_family(const s2attn_plan *plan, const s2attn_shape *shape, int alignment);
+
 int64_t s2attn_diff_backward_workspace_bytes(const s2attn_shape *shape);
 
 int s2attn_diff_backward(const void *k, const void *v, const void *q, const void *lam, int lam_dtype, const void *dy, const void *y, const void *y2, const float *lse,

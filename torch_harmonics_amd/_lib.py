@@ -153,6 +153,7 @@ SYMBOLS = {
     "s2attn_backward_dq": (_int, [_vp] * 7 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
     "s2attn_backward_dkdv": (_int, [_vp] * 8 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
     "s2attn_diff_forward": (_int, [_vp] * 4 + [_int] + [_vp] * 4 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
+    "s2attn_diff_family": (_int, [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _int]),
     "s2attn_diff_backward_workspace_bytes": (_i64, [ctypes.POINTER(ShapeStruct)]),
     "s2attn_diff_backward": (_int, [_vp] * 4 + [_int] + [_vp] * 10 + [ctypes.POINTER(PlanStruct), ctypes.POINTER(ShapeStruct), _vp]),
     "s2attn_group_norm_workspace_bytes": (_i64, [ctypes.POINTER(GroupNormStruct), _int]),

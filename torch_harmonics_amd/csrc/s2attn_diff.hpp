@@ -19,6 +19,7 @@ struct DArgs : Args {
     float *lam_part; // [B * nh][lam_n] summands of -dlam, written by the dq pass
     int lam_n;
     int lam_dtype;
+    int lam_blocks;  // leading workgroups of the dk/dv launch that sum dlam, a head each
 };
 
 __device__ inline float load_as_f32(const void *p, int i, int dtype)
@@ -209,10 +210,9 @@ template <typename T, int N> __device__ inline void diff_point_dkdv(const DArgs 
 }
 
 // dlam of one head from the summands that the dq pass left, in a fixed order, by one workgroup.  The summands of a head are added up in 64 bits:
-// there are up to millions of them, of both signs.
-__device__ inline void diff_sum_lam(const DArgs &a, int h, int tid, int nthreads)
+// there are up to millions of them, of both signs.  part: LDS, a number per wavefront.
+__device__ inline void diff_sum_lam(const DArgs &a, int h, int tid, int nthreads, double *part)
 {
-    __shared__ double part[16];
     double s = 0.0;
     for (int b = 0; b < a.B; b++) {
         const float *p = a.lam_part + (size_t)(b * a.nh + h) * a.lam_n;
@@ -238,10 +238,12 @@ __device__ inline void diff_sum_lam(const DArgs &a, int h, int tid, int nthreads
 
 // Workgroups of four points, as many as a launch of 2^31 threads has, each then the next four; the first `lam_blocks` workgroups of the dk/dv launch sum dlam, a head each.
 constexpr int DPT = 4;
-template <typename T, int N, Which PASS> __global__ __launch_bounds__(64 * DPT) void diff_points_kernel(const DArgs a, int lam_blocks, long npoints)
+template <typename T, int N, Which PASS> __global__ __launch_bounds__(64 * DPT) void diff_points_kernel(const DArgs a, long npoints)
 {
-    if (PASS == DKDV && (int)blockIdx.x < lam_blocks) {
-        diff_sum_lam(a, blockIdx.x, threadIdx.x, 64 * DPT);
+    const int lam_blocks = PASS == DKDV ? a.lam_blocks : 0;
+    if ((int)blockIdx.x < lam_blocks) {
+        __shared__ double part[DPT];
+        diff_sum_lam(a, blockIdx.x, threadIdx.x, 64 * DPT, part);
         return;
     }
     const int lane = threadIdx.x & 63;

@@ -1,0 +1,632 @@
+// Differential attention on 16-bit matrix instructions, 16-bit storage.  Included by s2attn_kernels.hip inside namespace s2 after s2attn_diff.hpp.
+//
+// Tiling, staging and the layout of scores as in s2attn_h16.hpp: a workgroup of four wavefronts owns 64 consecutive longitudes of one
+// latitude, 16 per wavefront, and walks its runs in steps of 32 band positions on one staged band of k and v (q and dy); lane l = (c = l %
+// 16, qd = l / 16); scores are produced transposed, S^T[position][column].
+//
+// The row of k (q) holds both maps' channels and is staged once; map i's scores take the 32-channel blocks it has channels in, with the other map's
+// channels zero on the side that stays in registers.  <dy, v>, the masks, the staged rows and the transposed reads of v serve both maps.
+// Sums of probabilities (forward) and of dS and of P (dq pass: the corrections of D, see diff_point_dq) are further products with the
+// staged rows or with ones, so they are of the rounded values that the other products take.
+//
+// Shape domain: ck a multiple of 8, cv a multiple of 8, 2 ck and cv at most D (a tile is D channels wide, 32, 64 or 128; zeros are staged past
+// a head's channels and never stored; PAD = false: 2 ck = cv = D), at least 32 columns per virtual latitude, rows 16-byte aligned.
+
+template <int D> struct DiffBand {
+    static constexpr int CPR = D / 8;                   // 16-byte pieces per row
+    static constexpr int PITCH = 2 * D + 32;            // bytes (32 or 96 modulo 128: free of bank conflicts, see WgBand)
+    static constexpr int RPI = 64 * NW / CPR;           // rows per iteration of the workgroup
+    static constexpr int NIT = (FRESH + RPI - 1) / RPI; // iterations for the first step of a run
+    static constexpr int BYTES = BR * PITCH;            // one tensor's ring
+    u4v ra[NIT], rb[NIT];
+
+    // N rows from longitude cs on (0 <= cs < W); lda, ldb: bytes between two columns; a_ok, b_ok: this thread's piece lies in the row
+    template <int N, bool PAD> __device__ inline void fetch(const char *pa, const char *pb, int tid, int cs, int W, unsigned lda, unsigned ldb, bool a_ok, bool b_ok)
+    {
+        const int r0 = tid / CPR;
+        const unsigned pc = 16u * (tid % CPR);
+#pragma unroll
+        for (int it = 0; it < (N + RPI - 1) / RPI; it++) {
+            if (PAD) ra[it] = u4v{0u, 0u, 0u, 0u}, rb[it] = u4v{0u, 0u, 0u, 0u};
+            if ((it + 1) * RPI <= N || it * RPI + r0 < N) {
+                unsigned col = (unsigned)(cs + r0); // r0 < RPI <= 64 <= 2 W
+                col = min(col, col - (unsigned)W);  // col - W wraps to a huge value when col < W
+                if (RPI > 32) col = min(col, col - (unsigned)W);
+                if (!PAD || a_ok) ra[it] = *reinterpret_cast<const u4v *>(pa + col * lda + pc);
+                if (!PAD || b_ok) rb[it] = *reinterpret_cast<const u4v *>(pb + col * ldb + pc);
+            }
+            cs += RPI;
+            while (cs >= W) cs -= W;
+        }
+    }
+    template <int N> __device__ inline void commit(char *A, char *B, int tid, int x0) const
+    {
+        const int r0 = tid / CPR, pc = 16 * (tid % CPR);
+#pragma unroll
+        for (int it = 0; it < (N + RPI - 1) / RPI; it++) {
+            if ((it + 1) * RPI <= N || it * RPI + r0 < N) {
+                const int o = ((x0 + it * RPI + r0) & (BR - 1)) * PITCH + pc;
+                *reinterpret_cast<u4v *>(A + o) = ra[it];
+                *reinterpret_cast<u4v *>(B + o) = rb[it];
+            }
+        }
+    }
+};
+template <int D> constexpr int d16_lds_bytes() { return 2 * DiffBand<D>::BYTES; }
+
+// The lane's own row of both maps (a query's q, or a key's k): op[i][s] = channels 32 s + 8 qd .. + 8 of its row that belong to map i, zeros elsewhere
+template <typename M, int D, bool PAD> struct DiffOwn {
+    static constexpr int NS = D / 32;
+    uint4 op[2][NS];
+    template <bool SCALED> __device__ inline void load(const char *row, int qd, int d)
+    {
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const int ch = 32 * s + 8 * qd;
+            uint4 x = h16_load_piece(row + 2 * ch, !PAD || ch < 2 * d);
+            if (SCALED) x = h16_scale_log2e<M>(x);
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            op[0][s] = ch < d ? x : zero;
+            op[1][s] = ch < d ? zero : x;
+        }
+    }
+    __device__ inline void settle_()
+    {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+                if (has(i, s)) settle(op[i][s]);
+    }
+    // does block s hold channels of map i?  (PAD: perhaps)
+    static constexpr __device__ bool has(int i, int s) { return PAD || D == 32 || (i == 0 ? s < NS / 2 : s >= NS / 2); }
+    // sc[i] += (16 staged rows) x own, both maps
+    __device__ inline void scores(f4v &s0, f4v &s1, const char *blk, int c, int qd, int d) const
+    {
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const uint4 x = h16_read_row<DiffBand<D>::PITCH>(blk, s, c, qd);
+            if (has(0, s) && (!PAD || 32 * s < d)) s0 = M::mfma(x, op[0][s], s0);
+            if (has(1, s) && (!PAD || (32 * s + 32 > d && 32 * s < 2 * d))) s1 = M::mfma(x, op[1][s], s1);
+        }
+    }
+};
+
+// Sums over positions of row[channel] * coefficient for rows of two maps: 16-channel block cb takes the coefficients of its map.  Where a block holds
+// channels of both (PAD with d an odd multiple of 8) it is computed with either, the second in `both`.
+template <typename M, int D, bool PAD> struct DiffSum {
+    static constexpr int NCB = D / 16;
+    f4v acc[NCB], both;
+    __device__ inline void zero()
+    {
+#pragma unroll
+        for (int cb = 0; cb < NCB; cb++) acc[cb] = f4v{0.f, 0.f, 0.f, 0.f};
+        both = f4v{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ inline void add(int cb, uint4 rows, uint4 p0, uint4 p1, int d)
+    {
+        if (!PAD) {
+            acc[cb] = M::mfma(rows, cb < NCB / 2 ? p0 : p1, acc[cb]);
+        } else if (16 * cb < d) {
+            acc[cb] = M::mfma(rows, p0, acc[cb]);
+            if (16 * cb + 16 > d) both = M::mfma(rows, p1, both);
+        } else if (16 * cb < 2 * d) {
+            acc[cb] = M::mfma(rows, p1, acc[cb]);
+        }
+    }
+    // of this lane's channels 16 cb + 4 qd .. + 4
+    __device__ inline f4v value(int cb, int qd, int d) const { return PAD && 16 * cb < d && 16 * cb + 4 * qd >= d ? both : acc[cb]; }
+    static __device__ inline bool first(int cb, int qd, int d) { return PAD ? 16 * cb + 4 * qd < d : cb < NCB / 2; }
+};
+
+template <typename M> __device__ inline uint4 d16_pack(const f4v (&x)[2])
+{
+    return make_uint4(M::pack2(x[0][0], x[0][1]), M::pack2(x[0][2], x[0][3]), M::pack2(x[1][0], x[1][1]), M::pack2(x[1][2], x[1][3]));
+}
+template <typename M> __device__ inline uint4 d16_ones()
+{
+    const unsigned one = M::pack2(1.f, 1.f);
+    return make_uint4(one, one, one, one);
+}
+
+// The kernel's arguments again and the lanes counted anew, as point_args() has it
+__device__ inline DArgs diff_point_args()
+{
+    typedef const int __attribute__((address_space(4))) * words;
+    words p = (words)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    DArgs a;
+    static_assert(sizeof(DArgs) % 4 == 0, "read as 32-bit words");
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(DArgs) / 4; i++) reinterpret_cast<int *>(&a)[i] = p[i];
+    return a;
+}
+// The columns `redo` of a wavefront whose sums are not finite, stored already
+template <typename T, int D, Which PASS> __device__ __forceinline__ void diff_redo(int wv, int block, unsigned redo)
+{
+    __threadfence(); // what is written here comes after it
+    const DArgs a = diff_point_args();
+    S2_H16_IDS_OF(64 * wv + point_lane(), block, PASS == DKDV ? a.Wi : a.Wo, PASS == DKDV ? a.Hi : a.Ho)
+    (void)c, (void)qd, (void)nvalid;
+    const int row = (PASS == DKDV ? a.sorder : a.gorder)[rowsel];
+    for (; redo; redo &= redo - 1) {
+        const int col = w0 + __builtin_ctz(redo);
+        if (PASS == FWD) diff_point_forward<T, D / 16>(a, b, h, bh, row, col, lane);
+        if (PASS == DQ) diff_point_dq<T, D / 16>(a, b, h, bh, row, col, lane);
+        if (PASS == DKDV) diff_point_dkdv<T, D / 16>(a, b, h, bh, row, col, lane);
+    }
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------------
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void fwd_d16_kernel(const DArgs a)
+{
+    typedef DiffBand<D> Tile;
+    typedef H16<T> M;
+    constexpr int PITCH = Tile::PITCH, NCB = D / 16;
+    extern __shared__ __attribute__((aligned(16))) char h16_lds[];
+    char *Ks = h16_lds, *Vs = h16_lds + Tile::BYTES;
+
+    S2_H16_IDS(a.Wo, a.Ho)
+    const int wv = __builtin_amdgcn_readfirstlane(wave);
+    const int ho = a.gorder[rowsel];
+    const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
+    const char *kx = static_cast<const char *>(a.k) + ((size_t)b * a.Hi * a.Wi * a.ldk + (size_t)h * nk) * 2;
+    const char *vx = static_cast<const char *>(a.v) + ((size_t)b * a.Hi * a.Wi * a.ldv + (size_t)h * nv) * 2;
+    const bool mine = c < nvalid;
+    const size_t pt = (size_t)query_point(a, b, ho, ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
+
+    DiffOwn<M, D, PAD> own;
+    own.template load<false>(static_cast<const char *>(a.q) + (pt * a.ldq + (size_t)h * nk) * 2, qd, d);
+    f4v acc[2][NCB], Z[2]; // Y^T of each map: register v of block cb is channel 16 cb + 4 qd + v of column c; sums of probabilities
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        Z[i] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int cb = 0; cb < NCB; cb++) acc[i][cb] = f4v{0.f, 0.f, 0.f, 0.f};
+    }
+    float m[2] = {NEG_BIG, NEG_BIG};
+    const uint4 ones = d16_ones<M>();
+
+    H16Walk wk;
+    wk.ri = a.goff[ho];
+    wk.rend = a.goff[ho + 1];
+    wk.pos = 0;
+    wk.run = Run{0, 0, 0, 0};
+    Tile bd;
+    const unsigned lda = 2u * a.ldk * a.kps, ldb = 2u * a.ldv * a.kps; // bytes between two columns of a virtual input latitude
+    const bool a_ok = 8 * (tid % Tile::CPR) < nk, b_ok = 8 * (tid % Tile::CPR) < nv;
+    auto fetch = [&](const Run &rn, bool fresh) {
+        const size_t row = (size_t)key_row(a, rn.lat, rn.pad);
+        const int cs = wk.stage(fresh, rn.ws + wg0, a.Wi);
+        if (fresh)
+            bd.template fetch<FRESH, PAD>(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, cs, a.Wi, lda, ldb, a_ok, b_ok);
+        else
+            bd.template fetch<HK, PAD>(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, cs, a.Wi, lda, ldb, a_ok, b_ok);
+    };
+    wk.w = 1.f;
+    if (wk.ri < wk.rend) {
+        wk.run = a.gruns[wk.ri];
+        wk.w = a.quad_w[wk.run.pad];
+        fetch(wk.run, true);
+        bd.template commit<FRESH>(Ks, Vs, tid, 0);
+    }
+    __syncthreads();
+    own.settle_();
+
+    while (wk.ri < wk.rend) {
+        wk.plan(a.gruns, a.quad_w);
+        if (wk.more) fetch(wk.nrun, wk.fresh);
+        if (active) {
+            const float lw = fast_log2(wk.w);
+            const int len = wk.run.len, pos = wk.pos;
+            const int xw = HQ * wave + pos; // band row of this wavefront's position `pos`
+            const char *kblk[2] = {band_block<PITCH>(Ks, xw), band_block<PITCH>(Ks, xw + 16)};
+            const char *vblk[2] = {band_block<PITCH>(Vs, xw), band_block<PITCH>(Vs, xw + 16)};
+            f4v sc[2][2]; // [map][block]
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) {
+                sc[0][kb] = sc[1][kb] = f4v{0.f, 0.f, 0.f, 0.f};
+                own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd, d);
+            }
+            const int tb = pos + 4 * qd - c; // neighbor index of element (kb, v): tb + 16 kb + v
+            if (!(pos >= HQ - 1 && pos + HK <= len)) {
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const bool in = (unsigned)(tb + 16 * kb + v) < (unsigned)len;
+                        sc[0][kb][v] = in ? sc[0][kb][v] : -INFINITY;
+                        sc[1][kb][v] = in ? sc[1][kb][v] : -INFINITY;
+                    }
+            }
+            float mx[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                mx[i] = fmaxf(fmaxf(fmaxf(sc[i][0][0], sc[i][0][1]), fmaxf(sc[i][0][2], sc[i][0][3])), fmaxf(fmaxf(sc[i][1][0], sc[i][1][1]), fmaxf(sc[i][1][2], sc[i][1][3])));
+            // The running maxima are only the reference points of the exponentials: see fwd_h16_kernel.
+            if (__any(fmaf(mx[0], LOG2E, lw) > m[0] + RESCALE_THR || fmaf(mx[1], LOG2E, lw) > m[1] + RESCALE_THR)) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float cm = fmaf(h16_quarter_max(mx[i]), LOG2E, lw);
+                    const float mn = (cm > m[i] + RESCALE_THR) ? cm : m[i]; // m starts finite, so mn is finite
+                    const float corr = fast_exp2(m[i] - mn);
+                    Z[i] *= corr;
+#pragma unroll
+                    for (int cb = 0; cb < NCB; cb++) acc[i][cb] *= corr;
+                    m[i] = mn;
+                }
+            }
+            uint4 p[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float sh = lw - m[i];
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) sc[i][kb][v] = fast_exp2(fmaf(sc[i][kb][v], LOG2E, sh)); // masked: exp2(-inf) = 0
+                p[i] = d16_pack<M>(sc[i]);
+                Z[i] = M::mfma(ones, p[i], Z[i]);
+            }
+#pragma unroll
+            for (int cb = 0; cb < NCB; cb++) {
+                const uint4 vt = h16_read_transposed<PITCH>(vblk[0], vblk[1], cb, c, qd);
+                acc[0][cb] = M::mfma(vt, p[0], acc[0][cb]);
+                acc[1][cb] = M::mfma(vt, p[1], acc[1][cb]);
+            }
+        }
+        if (wk.more) {
+            if (wk.fresh) {
+                __syncthreads(); // the next run's rows replace rows the slowest wavefront may still be reading
+                bd.template commit<FRESH>(Ks, Vs, tid, 0);
+            } else {
+                bd.template commit<HK>(Ks, Vs, tid, FRESH - HK + wk.npos);
+            }
+        }
+        __syncthreads();
+        wk.advance();
+    }
+
+    float check = Z[0][0] + Z[1][0];
+#pragma unroll
+    for (int cb = 0; cb < NCB; cb++) check += point_sum(acc[0][cb] + acc[1][cb]);
+    const unsigned redo = point_columns(mine && not_finite(check));
+    if (mine) {
+        const float z0 = Z[0][0], z1 = Z[1][0];
+        if (a.lse2 && qd == 0)
+            a.lse2[((size_t)bh * a.Ho + ho) * a.Wo + w0 + c] = make_float2(z0 == 0.f ? INFINITY : m[0] + fast_log2(z0), z1 == 0.f ? INFINITY : m[1] + fast_log2(z1));
+        const float i0 = z0 == 0.f ? 0.f : 1.0f / z0, i1 = z1 == 0.f ? 0.f : 1.0f / z1, lam = load_as_f32(a.lam, h, a.lam_dtype);
+        char *y = static_cast<char *>(a.y) + (pt * a.ldy + (size_t)h * nv + 4 * qd) * 2;
+        char *y2 = static_cast<char *>(a.y2) + ((pt * a.nh + h) * nv + 4 * qd) * 2;
+#pragma unroll
+        for (int cb = 0; cb < NCB; cb++)
+            if (!PAD || 16 * cb + 4 * qd < nv) {
+                const f4v o2 = acc[1][cb] * i1, o = acc[0][cb] * i0 - lam * o2;
+                *reinterpret_cast<uint2 *>(y + 32 * cb) = make_uint2(M::pack2(o[0], o[1]), M::pack2(o[2], o[3]));
+                if (a.y2) *reinterpret_cast<uint2 *>(y2 + 32 * cb) = make_uint2(M::pack2(o2[0], o2[1]), M::pack2(o2[2], o2[3]));
+            }
+    }
+    if (__builtin_expect(redo != 0, 0)) diff_redo<T, D, FWD>(wv, blockIdx.x, redo);
+}
+
+// ---- backward, dq pass -----------------------------------------------------------------------------------------------------------
+// Per step and map S^T = K Q^T; G^T = V dY^T once; dQ^T += K^T dS^T, and AK^T += K^T P^T and sum dS for the corrections of D.
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void dq_d16_kernel(const DArgs a)
+{
+    typedef DiffBand<D> Tile;
+    typedef H16<T> M;
+    constexpr int PITCH = Tile::PITCH, NS = D / 32, NCB = D / 16;
+    extern __shared__ __attribute__((aligned(16))) char h16_lds[];
+    char *Ks = h16_lds, *Vs = h16_lds + Tile::BYTES;
+
+    S2_H16_IDS(a.Wo, a.Ho)
+    const int wv = __builtin_amdgcn_readfirstlane(wave);
+    const int ho = a.gorder[rowsel];
+    const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
+    const char *kx = static_cast<const char *>(a.k) + ((size_t)b * a.Hi * a.Wi * a.ldk + (size_t)h * nk) * 2;
+    const char *vx = static_cast<const char *>(a.v) + ((size_t)b * a.Hi * a.Wi * a.ldv + (size_t)h * nv) * 2;
+    const bool mine = c < nvalid;
+    const size_t pt = (size_t)query_point(a, b, ho, ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
+    const size_t sidx = ((size_t)bh * a.Ho + ho) * a.Wo + w0 + (mine ? c : 0);
+    const float lam = load_as_f32(a.lam, h, a.lam_dtype);
+
+    DiffOwn<M, D, PAD> own; // q log2 e
+    own.template load<true>(static_cast<const char *>(a.q) + (pt * a.ldq + (size_t)h * nk) * 2, qd, d);
+    uint4 gop[NS];
+    float D1 = 0.f, D2 = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+        const bool ok = !PAD || 32 * s + 8 * qd < nv;
+        const size_t off = 16 * qd + 64 * s;
+        gop[s] = h16_load_piece(static_cast<const char *>(a.dy) + (pt * a.ldg + (size_t)h * nv) * 2 + off, ok);
+        const uint4 yv = h16_load_piece(static_cast<const char *>(a.ysaved) + (pt * a.ldy + (size_t)h * nv) * 2 + off, ok);
+        const uint4 y2 = h16_load_piece(static_cast<const char *>(a.y2saved) + (pt * a.nh + h) * nv * 2 + off, ok);
+        const unsigned gu[4] = {gop[s].x, gop[s].y, gop[s].z, gop[s].w}, yu[4] = {yv.x, yv.y, yv.z, yv.w}, y2u[4] = {y2.x, y2.y, y2.z, y2.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 g_ = M::unpack2(gu[i]), y_ = M::unpack2(yu[i]), y2_ = M::unpack2(y2u[i]);
+            D1 = fmaf(g_.x, y_.x, D1), D1 = fmaf(g_.y, y_.y, D1);
+            D2 = fmaf(g_.x, y2_.x, D2), D2 = fmaf(g_.y, y2_.y, D2);
+        }
+    }
+    D2 = h16_quarter_sum(D2);
+    D1 = fmaf(lam, D2, h16_quarter_sum(D1));
+    float2 lse = a.lse2[sidx];
+
+    DiffSum<M, D, PAD> acc, ak;
+    acc.zero(), ak.zero();
+    f4v off[2] = {f4v{0.f, 0.f, 0.f, 0.f}, f4v{0.f, 0.f, 0.f, 0.f}};
+    const uint4 ones = d16_ones<M>();
+
+    H16Walk wk;
+    wk.ri = a.goff[ho];
+    wk.rend = a.goff[ho + 1];
+    wk.pos = 0;
+    wk.run = Run{0, 0, 0, 0};
+    Tile bd;
+    const unsigned lda = 2u * a.ldk * a.kps, ldb = 2u * a.ldv * a.kps;
+    const bool a_ok = 8 * (tid % Tile::CPR) < nk, b_ok = 8 * (tid % Tile::CPR) < nv;
+    auto fetch = [&](const Run &rn, bool fresh) {
+        const size_t row = (size_t)key_row(a, rn.lat, rn.pad);
+        const int cs = wk.stage(fresh, rn.ws + wg0, a.Wi);
+        if (fresh)
+            bd.template fetch<FRESH, PAD>(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, cs, a.Wi, lda, ldb, a_ok, b_ok);
+        else
+            bd.template fetch<HK, PAD>(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, cs, a.Wi, lda, ldb, a_ok, b_ok);
+    };
+    wk.w = 1.f;
+    if (wk.ri < wk.rend) {
+        wk.run = a.gruns[wk.ri];
+        wk.w = a.quad_w[wk.run.pad];
+        fetch(wk.run, true);
+        bd.template commit<FRESH>(Ks, Vs, tid, 0);
+    }
+    __syncthreads();
+    own.settle_();
+    settle(gop);
+    settle(lse.x), settle(lse.y);
+    const float step21 = D1 - D2; // g - D2 = (g - D1) + (D1 - D2)
+
+    while (wk.ri < wk.rend) {
+        wk.plan(a.gruns, a.quad_w);
+        if (wk.more) fetch(wk.nrun, wk.fresh);
+        if (active) {
+            const float lw = fast_log2(wk.w), l0 = lw - lse.x, l1 = lw - lse.y;
+            const int len = wk.run.len, pos = wk.pos;
+            const int xw = HQ * wave + pos; // band row of this wavefront's position `pos`
+            const char *kblk[2] = {band_block<PITCH>(Ks, xw), band_block<PITCH>(Ks, xw + 16)};
+            const char *vblk[2] = {band_block<PITCH>(Vs, xw), band_block<PITCH>(Vs, xw + 16)};
+            // The accumulators start at log2 w - lse and at -D1, so the matrix cores hand back the exponents of p and g - D1.
+            f4v sc[2][2], gc[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) {
+                sc[0][kb] = f4v{l0, l0, l0, l0};
+                sc[1][kb] = f4v{l1, l1, l1, l1};
+                gc[kb] = f4v{-D1, -D1, -D1, -D1};
+                own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd, d);
+#pragma unroll
+                for (int s = 0; s < NS; s++) gc[kb] = M::mfma(h16_read_row<PITCH>(vblk[kb], s, c, qd), gop[s], gc[kb]);
+            }
+            const int tb = pos + 4 * qd - c;
+            const bool inner = pos >= HQ - 1 && pos + HK <= len; // every element of the step is a neighbor: no band mask
+            f4v ds[2][2];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const bool in = inner || (unsigned)(tb + 16 * kb + v) < (unsigned)len;
+                    sc[0][kb][v] = in ? fast_exp2(sc[0][kb][v]) : 0.f;
+                    sc[1][kb][v] = in ? fast_exp2(sc[1][kb][v]) : 0.f;
+                    ds[0][kb][v] = sc[0][kb][v] * gc[kb][v];
+                    ds[1][kb][v] = sc[1][kb][v] * (gc[kb][v] + step21);
+                }
+            const uint4 p0 = d16_pack<M>(sc[0]), p1 = d16_pack<M>(sc[1]), d0 = d16_pack<M>(ds[0]), d1 = d16_pack<M>(ds[1]);
+            off[0] = M::mfma(ones, d0, off[0]);
+            off[1] = M::mfma(ones, d1, off[1]);
+#pragma unroll
+            for (int cb = 0; cb < NCB; cb++) {
+                const uint4 kt = h16_read_transposed<PITCH>(kblk[0], kblk[1], cb, c, qd);
+                acc.add(cb, kt, d0, d1, d);
+                ak.add(cb, kt, p0, p1, d);
+            }
+        }
+        if (wk.more) {
+            if (wk.fresh) {
+                __syncthreads(); // the next run's rows replace rows the slowest wavefront may still be reading
+                bd.template commit<FRESH>(Ks, Vs, tid, 0);
+            } else {
+                bd.template commit<HK>(Ks, Vs, tid, FRESH - HK + wk.npos);
+            }
+        }
+        __syncthreads();
+        wk.advance();
+    }
+
+    // (stored after the walk: a global store ahead of the loop would turn the loop's scalar loads of runs and weights,
+    // which the compiler only uses while nothing in the kernel can have written memory, into vector loads with waits)
+    const float o0 = off[0][0], o1 = off[1][0];
+    float check = o0 + o1;
+#pragma unroll
+    for (int cb = 0; cb < NCB; cb++) check += point_sum(acc.acc[cb] + ak.acc[cb]);
+    if (PAD) check += point_sum(acc.both + ak.both);
+    const unsigned redo = point_columns(mine && not_finite(check));
+    float part = 0.f;
+    if (mine) {
+        // (a column that is evaluated again may hold a value here that it does not see)
+        const float s2 = not_finite(o1) ? D2 : D2 + o1;
+        part = qd == 0 ? s2 : 0.f;
+        if (qd == 0) a.dstats[sidx] = make_float4(lse.x, lse.y, D1 + o0, s2);
+        char *dq = static_cast<char *>(a.dq) + (pt * a.lddq + (size_t)h * nk + 4 * qd) * 2;
+#pragma unroll
+        for (int cb = 0; cb < NCB; cb++)
+            if (!PAD || 16 * cb + 4 * qd < nk) {
+                const bool first = acc.first(cb, qd, d);
+                f4v x = acc.value(cb, qd, d) - (first ? o0 : o1) * ak.value(cb, qd, d);
+                x *= first ? 1.f : -lam;
+                *reinterpret_cast<uint2 *>(dq + 32 * cb) = make_uint2(M::pack2(x[0], x[1]), M::pack2(x[2], x[3]));
+            }
+    }
+    if (active) {
+        part = point_lanes_sum(part);
+        if (lane == 0) a.lam_part[(size_t)bh * a.lam_n + (size_t)ho * ((a.Wo + HQ - 1) / HQ) + w0 / HQ] = part;
+    }
+    if (__builtin_expect(redo != 0, 0)) diff_redo<T, D, DQ>(wv, blockIdx.x, redo);
+}
+
+// ---- backward, dk/dv pass: transposed gather (see dkdv_h16_kernel) -------------------------------------------------------------------
+// Per step and map S = Q K^T; G = dY V^T once; dV^T += dY^T (P1 - lam P2) once; dK^T += Q^T dS.
+// The statistics of the staged queries lie in the padding of the rings' rows 4 j: log2 w - lse of the two maps for rows 4 j .. + 4 in that of Q, -D1
+// and D1 - D2 in that of dY, so a lane reads them as start values of its accumulators.
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void dkdv_d16_kernel(const DArgs a)
+{
+    typedef DiffBand<D> Tile;
+    typedef H16<T> M;
+    constexpr int PITCH = Tile::PITCH, NS = D / 32, NCB = D / 16;
+    extern __shared__ __attribute__((aligned(16))) char h16_lds[];
+    char *Qs = h16_lds, *Gs = h16_lds + Tile::BYTES;
+    constexpr int STAT = 2 * D;
+    if ((int)blockIdx.x < a.lam_blocks) {
+        diff_sum_lam(a, blockIdx.x, threadIdx.x, 64 * NW, reinterpret_cast<double *>(h16_lds));
+        return;
+    }
+    const int block = blockIdx.x - a.lam_blocks;
+
+    S2_H16_IDS_OF(threadIdx.x, block, a.Wi, a.Hi)
+    const int wv = __builtin_amdgcn_readfirstlane(wave);
+    const int hi = a.sorder[rowsel];
+    const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
+    const char *qy = static_cast<const char *>(a.q) + ((size_t)b * a.Ho * a.Wo * a.ldq + (size_t)h * nk) * 2;
+    const char *gy = static_cast<const char *>(a.dy) + ((size_t)b * a.Ho * a.Wo * a.ldg + (size_t)h * nv) * 2;
+    const float4 *stats = a.dstats + (size_t)bh * a.Ho * a.Wo;
+    const bool mine = c < nvalid;
+    const size_t pt = (size_t)key_point(a, b, hi, hi / a.kps) + (size_t)(w0 + (mine ? c : 0)) * a.kps;
+    float lam = load_as_f32(a.lam, h, a.lam_dtype);
+
+    DiffOwn<M, D, PAD> own; // k log2 e
+    own.template load<true>(static_cast<const char *>(a.k) + (pt * a.ldk + (size_t)h * nk) * 2, qd, d);
+    uint4 vop[NS];
+#pragma unroll
+    for (int s = 0; s < NS; s++) vop[s] = h16_load_piece(static_cast<const char *>(a.v) + (pt * a.ldv + (size_t)h * nv) * 2 + 16 * qd + 64 * s, !PAD || 32 * s + 8 * qd < nv);
+    DiffSum<M, D, PAD> dkt;
+    dkt.zero();
+    f4v dvt[NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; cb++) dvt[cb] = f4v{0.f, 0.f, 0.f, 0.f};
+    const float lw = fast_log2(a.quad_w[hi / a.kps]);
+
+    H16Walk wk;
+    wk.ri = a.soff[hi];
+    wk.rend = a.soff[hi + 1];
+    wk.pos = 0;
+    wk.run = Run{0, 0, 0, 0};
+    wk.w = 1.f;
+    Tile bd;
+    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+    const unsigned lda = 2u * a.ldq * a.qps, ldb = 2u * a.ldg * a.qps; // bytes between two columns of a virtual output latitude
+    const bool a_ok = 8 * (tid % Tile::CPR) < nk, b_ok = 8 * (tid % Tile::CPR) < nv;
+    auto fetch = [&](const Run &rn, bool fresh) {
+        int c0 = 0;
+        if (fresh) { // longitude of band row 0, in [0, 2 W)
+            c0 = wg0 - rn.ws - rn.len + 1 + a.Wo;
+            while (c0 < 0) c0 += a.Wo;
+        }
+        const int cs = wk.stage(fresh, c0, a.Wo);
+        const size_t row = (size_t)query_row(a, rn.lat, rn.pad);
+        if (fresh)
+            bd.template fetch<FRESH, PAD>(qy + 2 * row * a.ldq, gy + 2 * row * a.ldg, tid, cs, a.Wo, lda, ldb, a_ok, b_ok);
+        else
+            bd.template fetch<HK, PAD>(qy + 2 * row * a.ldq, gy + 2 * row * a.ldg, tid, cs, a.Wo, lda, ldb, a_ok, b_ok);
+        if (tid < (fresh ? FRESH : HK)) { // the first threads fetch the statistics of the staged rows
+            int col = cs + tid;
+            while (col >= a.Wo) col -= a.Wo;
+            st = stats[(size_t)rn.lat * a.Wo + col];
+        }
+    };
+    auto commit = [&](int x0) {
+        if (x0 == 0)
+            bd.template commit<FRESH>(Qs, Gs, tid, 0);
+        else
+            bd.template commit<HK>(Qs, Gs, tid, x0);
+        if (tid < (x0 == 0 ? FRESH : HK)) {
+            const int o = ((x0 + tid) & (BR - 4)) * PITCH + STAT + 4 * (tid & 3);
+            *reinterpret_cast<float *>(Qs + o) = lw - st.x;
+            *reinterpret_cast<float *>(Qs + o + 16) = lw - st.y;
+            *reinterpret_cast<float *>(Gs + o) = -st.z;
+            *reinterpret_cast<float *>(Gs + o + 16) = st.z - st.w;
+        }
+    };
+    if (wk.ri < wk.rend) {
+        wk.run = a.sruns[wk.ri];
+        fetch(wk.run, true);
+        commit(0);
+    }
+    __syncthreads();
+    own.settle_();
+    settle(vop);
+    settle(lam);
+
+    while (wk.ri < wk.rend) {
+        wk.plan(a.sruns);
+        if (wk.more) fetch(wk.nrun, wk.fresh);
+        if (active) {
+            const int len = wk.run.len, pos = wk.pos;
+            const int xw = HQ * wave + pos; // band row of this wavefront's position `pos`
+            const char *qblk[2] = {band_block<PITCH>(Qs, xw), band_block<PITCH>(Qs, xw + 16)};
+            const char *gblk[2] = {band_block<PITCH>(Gs, xw), band_block<PITCH>(Gs, xw + 16)};
+            f4v sc[2][2], gc[2], step[2];
+#pragma unroll
+            for (int qb = 0; qb < 2; qb++) {
+                const char *sq = qblk[qb] + 4 * qd * PITCH + STAT, *sg = gblk[qb] + 4 * qd * PITCH + STAT;
+                sc[0][qb] = *reinterpret_cast<const f4v *>(sq);
+                sc[1][qb] = *reinterpret_cast<const f4v *>(sq + 16);
+                gc[qb] = *reinterpret_cast<const f4v *>(sg);
+                step[qb] = *reinterpret_cast<const f4v *>(sg + 16);
+                own.scores(sc[0][qb], sc[1][qb], qblk[qb], c, qd, d);
+#pragma unroll
+                for (int s = 0; s < NS; s++) gc[qb] = M::mfma(h16_read_row<PITCH>(gblk[qb], s, c, qd), vop[s], gc[qb]);
+            }
+            const int tb = pos + 4 * qd - c; // r - c of element (qb, v): tb + 16 qb + v
+            const bool inner = pos >= HQ - 1 && pos + HK <= len; // every element of the step is a (query, key) pair of the run
+            f4v ds[2][2], co[2];
+#pragma unroll
+            for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const bool in = inner || (unsigned)(tb + 16 * qb + v) < (unsigned)len;
+                    const float p0 = in ? fast_exp2(sc[0][qb][v]) : 0.f, p1 = in ? fast_exp2(sc[1][qb][v]) : 0.f;
+                    co[qb][v] = fmaf(-lam, p1, p0);
+                    ds[0][qb][v] = p0 * gc[qb][v];
+                    ds[1][qb][v] = p1 * (gc[qb][v] + step[qb][v]);
+                }
+            const uint4 cop = d16_pack<M>(co), d0 = d16_pack<M>(ds[0]), d1 = d16_pack<M>(ds[1]);
+#pragma unroll
+            for (int cb = 0; cb < NCB; cb++) {
+                dvt[cb] = M::mfma(h16_read_transposed<PITCH>(gblk[0], gblk[1], cb, c, qd), cop, dvt[cb]);
+                dkt.add(cb, h16_read_transposed<PITCH>(qblk[0], qblk[1], cb, c, qd), d0, d1, d);
+            }
+        }
+        if (wk.more) {
+            if (wk.fresh) __syncthreads(); // the next run's rows replace rows the slowest wavefront may still be reading
+            commit(wk.fresh ? 0 : FRESH - HK + wk.npos);
+        }
+        __syncthreads();
+        wk.advance();
+    }
+
+    float check = 0.f;
+#pragma unroll
+    for (int cb = 0; cb < NCB; cb++) check += point_sum(dkt.acc[cb] + dvt[cb]);
+    if (PAD) check += point_sum(dkt.both);
+    const unsigned redo = point_columns(mine && not_finite(check));
+    if (mine) {
+        char *dk = static_cast<char *>(a.dk) + (pt * a.lddk + (size_t)h * nk + 4 * qd) * 2, *dv = static_cast<char *>(a.dv) + (pt * a.lddv + (size_t)h * nv + 4 * qd) * 2;
+#pragma unroll
+        for (int cb = 0; cb < NCB; cb++) {
+            if (!PAD || 16 * cb + 4 * qd < nk) {
+                const f4v x = dkt.value(cb, qd, d) * (dkt.first(cb, qd, d) ? 1.f : -lam);
+                *reinterpret_cast<uint2 *>(dk + 32 * cb) = make_uint2(M::pack2(x[0], x[1]), M::pack2(x[2], x[3]));
+            }
+            if (!PAD || 16 * cb + 4 * qd < nv) *reinterpret_cast<uint2 *>(dv + 32 * cb) = make_uint2(M::pack2(dvt[cb][0], dvt[cb][1]), M::pack2(dvt[cb][2], dvt[cb][3]));
+        }
+    }
+    if (__builtin_expect(redo != 0, 0)) diff_redo<T, D, DKDV>(wv, block, redo);
+}

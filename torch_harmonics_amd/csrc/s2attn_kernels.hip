@@ -36,11 +36,11 @@
 
 #include "s2attn_internal.h"
 
-// This file is compiled seven times (see the Makefile), so that the groups of kernel instantiations build side by
+// This file is compiled eight times (see the Makefile), so that the groups of kernel instantiations build side by
 // side: S2_PART 1 = everything but the launchers of the 16-longitude matrix-core families, 2 = the 16-bit family
 // (s2attn_h16.hpp), 3 = the fp32 family (s2attn_m32.hpp), 4 = its ring-step kernels for 16-bit storage, 5 = the split-product family
 // (s2attn_s16.hpp), 6 = its ring steps
-// (s2attn_s16_ring.hpp), 7 = differential attention one point at a time (s2attn_diff.hpp).  S2_PART 0 (the default) is the whole library in one unit.
+// (s2attn_s16_ring.hpp), 7 = differential attention one point at a time (s2attn_diff.hpp), 8 = in 16-bit tiles (s2attn_diff16.hpp).  S2_PART 0 (the default) is the whole library in one unit.
 #ifndef S2_PART
 #define S2_PART 0
 #endif
@@ -2284,6 +2284,7 @@ template <typename T> __global__ __launch_bounds__(64) void dkdv_mfma_kernel(con
 #include "s2attn_s16.hpp"
 #include "s2attn_s16_ring.hpp"
 #include "s2attn_diff.hpp"
+#include "s2attn_diff16.hpp"
 
 // ---------------------------------------------------------------------------------
 // layout permutes: batched 2-D transpose [R, S] -> [S, R] through a 64x65 LDS tile
@@ -2323,6 +2324,7 @@ template <typename T, int D, bool PAD, int MODE> int launch_ring_s16(const Args 
 template <int D, int MODE, typename T> int launch_ring_m32(const Args &a0, hipStream_t stream);
 template <int D, bool WRITE, typename T> int launch_ring_pass2_m32(const Args &a0, hipStream_t stream);
 template <typename T> int launch_diff_points(Which which, const DArgs &a, hipStream_t stream);
+template <typename T, int D, bool PAD> int launch_d16(Which which, const DArgs &a, hipStream_t stream);
 
 #if S2_PART == 0 || S2_PART == 2
 // 16-bit matrix-core kernels: bf16 / fp16 storage, head dim D, equal longitude counts, 16-byte aligned tensors.  The
@@ -2566,11 +2568,10 @@ template int launch_ring_m32<128, 2, f16_t>(const Args &, hipStream_t);
 template <typename T, int N> int launch_diff_points_n(Which which, const DArgs &a, hipStream_t stream)
 {
     const long points = (which == DKDV ? (a.dk ? (long)a.Hi * a.Wi : 0) : (long)a.Ho * a.Wo) * a.B * a.nh;
-    const int lam_blocks = which == DKDV && a.dlam ? a.nh : 0;
-    const long nblocks = lam_blocks + std::min((points + DPT - 1) / DPT, 1L << 23);
+    const long nblocks = (which == DKDV ? a.lam_blocks : 0) + std::min((points + DPT - 1) / DPT, 1L << 23);
     if (nblocks == 0) return S2ATTN_OK;
-    void (*const kern)(const DArgs, int, long) = which == FWD ? diff_points_kernel<T, N, FWD> : which == DQ ? diff_points_kernel<T, N, DQ> : diff_points_kernel<T, N, DKDV>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(64 * DPT), 0, stream, a, lam_blocks, points);
+    void (*const kern)(const DArgs, long) = which == FWD ? diff_points_kernel<T, N, FWD> : which == DQ ? diff_points_kernel<T, N, DQ> : diff_points_kernel<T, N, DKDV>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(64 * DPT), 0, stream, a, points);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return s2attn_fail(S2ATTN_E_LAUNCH, "kernel launch: %s", hipGetErrorString(e));
     return S2ATTN_OK;
@@ -2588,6 +2589,41 @@ template <typename T> int launch_diff_points(Which which, const DArgs &a, hipStr
 template int launch_diff_points<float>(Which, const DArgs &, hipStream_t);
 template int launch_diff_points<bf16_t>(Which, const DArgs &, hipStream_t);
 template int launch_diff_points<f16_t>(Which, const DArgs &, hipStream_t);
+#endif
+// differential attention, tiles of 64 columns
+template <typename K> int launch_diff_tiles(K kern, Which which, const DArgs &a, int lds, hipStream_t stream)
+{
+    const long tiles = (which == DKDV ? (a.dk ? (long)a.Hi * ((a.Wi + WQ - 1) / WQ) : 0) : (long)a.Ho * ((a.Wo + WQ - 1) / WQ)) * a.B * a.nh;
+    const long nblocks = tiles + (which == DKDV ? a.lam_blocks : 0);
+    if (nblocks >= (1L << 32) / (64 * NW)) return s2attn_fail(S2ATTN_E_UNSUPPORTED, "problem needs %ld workgroups, more than one grid holds", nblocks);
+    if (nblocks == 0) return S2ATTN_OK;
+    if (lds > 48 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return s2attn_fail(S2ATTN_E_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(64 * NW), lds, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return s2attn_fail(S2ATTN_E_LAUNCH, "kernel launch: %s", hipGetErrorString(e));
+    return S2ATTN_OK;
+}
+#if S2_PART == 0 || S2_PART == 8
+template <typename T, int D, bool PAD> int launch_d16(Which which, const DArgs &a, hipStream_t stream)
+{
+    void (*const kern)(const DArgs) = which == FWD ? fwd_d16_kernel<T, D, PAD> : which == DQ ? dq_d16_kernel<T, D, PAD> : dkdv_d16_kernel<T, D, PAD>;
+    return launch_diff_tiles(kern, which, a, d16_lds_bytes<D>(), stream);
+}
+#endif
+#if S2_PART == 8
+#define S2_D16_INSTANCES(T)                                                    \
+    template int launch_d16<T, 32, false>(Which, const DArgs &, hipStream_t);  \
+    template int launch_d16<T, 64, false>(Which, const DArgs &, hipStream_t);  \
+    template int launch_d16<T, 128, false>(Which, const DArgs &, hipStream_t); \
+    template int launch_d16<T, 32, true>(Which, const DArgs &, hipStream_t);   \
+    template int launch_d16<T, 64, true>(Which, const DArgs &, hipStream_t);   \
+    template int launch_d16<T, 128, true>(Which, const DArgs &, hipStream_t);
+S2_D16_INSTANCES(bf16_t)
+S2_D16_INSTANCES(f16_t)
+#undef S2_D16_INSTANCES
 #endif
 } // namespace s2
 
@@ -3408,14 +3444,47 @@ int diff_args(DArgs &a, const void *k, const void *v, const void *q, const void 
     a.k = k, a.v = v, a.q = q, a.lam = lam, a.lam_dtype = lam_dtype;
     return S2ATTN_OK;
 }
-template <typename T> int launch_diff_t(Which which, DArgs &a, hipStream_t stream)
+// The kernels that take a problem: one decision for all passes of a call, from the shape and the alignment of its tensors.
+template <typename T> int diff_family_t(const DArgs &a, size_t alignment)
 {
+    const int c = std::max(a.dk_, a.dv_);
+    if (a.Wi < HK) return S2ATTN_FAMILY_VECTOR;
+    if constexpr (!std::is_same<T, float>::value) {
+        const bool strides = (a.ldk | a.ldv | a.ldq | a.ldy | a.ldg | a.lddk | a.lddv | a.lddq) % 8 == 0;
+        if (a.dk_ % 16 == 0 && a.dv_ % 8 == 0 && c <= 128 && strides && alignment % 16 == 0) return S2ATTN_FAMILY_16BIT;
+    }
+    return S2ATTN_FAMILY_VECTOR;
+}
+int diff_family(const DArgs &a, int dtype, size_t alignment)
+{
+    if (dtype == S2ATTN_F32) return diff_family_t<float>(a, alignment);
+    return dtype == S2ATTN_BF16 ? diff_family_t<bf16_t>(a, alignment) : diff_family_t<f16_t>(a, alignment);
+}
+size_t common_alignment(std::initializer_list<const void *> ptrs)
+{
+    size_t bits = 0;
+    for (const void *p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
+    return bits ? bits & (~bits + 1) : 4096;
+}
+template <typename T> int launch_diff_t(Which which, int family, DArgs &a, hipStream_t stream)
+{
+    a.lam_n = a.Ho * (family == S2ATTN_FAMILY_VECTOR ? a.Wo : (a.Wo + HQ - 1) / HQ);
+    a.lam_blocks = which == DKDV && a.dlam ? a.nh : 0;
+    if constexpr (!std::is_same<T, float>::value) {
+        if (family == S2ATTN_FAMILY_16BIT) {
+            const int c = std::max(a.dk_, a.dv_);
+            const bool exact = a.dk_ == a.dv_;
+            if (c <= 32) return exact && c == 32 ? launch_d16<T, 32, false>(which, a, stream) : launch_d16<T, 32, true>(which, a, stream);
+            if (c <= 64) return exact && c == 64 ? launch_d16<T, 64, false>(which, a, stream) : launch_d16<T, 64, true>(which, a, stream);
+            return exact && c == 128 ? launch_d16<T, 128, false>(which, a, stream) : launch_d16<T, 128, true>(which, a, stream);
+        }
+    }
     return launch_diff_points<T>(which, a, stream);
 }
-int launch_diff(Which which, DArgs &a, int dtype, hipStream_t stream)
+int launch_diff(Which which, int family, DArgs &a, int dtype, hipStream_t stream)
 {
-    if (dtype == S2ATTN_F32) return launch_diff_t<float>(which, a, stream);
-    return dtype == S2ATTN_BF16 ? launch_diff_t<bf16_t>(which, a, stream) : launch_diff_t<f16_t>(which, a, stream);
+    if (dtype == S2ATTN_F32) return launch_diff_t<float>(which, family, a, stream);
+    return dtype == S2ATTN_BF16 ? launch_diff_t<bf16_t>(which, family, a, stream) : launch_diff_t<f16_t>(which, family, a, stream);
 }
 } // namespace
 
@@ -3429,7 +3498,17 @@ extern "C" int s2attn_diff_forward(const void *k, const void *v, const void *q, 
     if (!y2 != !lse) return s2attn_fail(S2ATTN_E_INVALID, "y2 and lse are kept together or not at all");
     if (lse && !aligned(lse, sizeof(float2))) return s2attn_fail(S2ATTN_E_INVALID, "lse must be 8-byte aligned");
     a.y = y, a.y2 = y2, a.lse2 = reinterpret_cast<float2 *>(lse);
-    return launch_diff(FWD, a, shape->dtype, static_cast<hipStream_t>(stream));
+    return launch_diff(FWD, diff_family(a, shape->dtype, common_alignment({k, v, q, y, y2})), a, shape->dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int s2attn_diff_family(const s2attn_plan *plan, const s2attn_shape *shape, int alignment)
+{
+    DArgs a = {};
+    float *const at = reinterpret_cast<float *>((uintptr_t)16); // (not looked at)
+    const int rc = diff_args(a, at, at, at, at, S2ATTN_F32, at, plan, shape);
+    if (rc != S2ATTN_OK) return rc;
+    if (alignment < 1) return s2attn_fail(S2ATTN_E_INVALID, "the alignment is at least 1");
+    return diff_family(a, shape->dtype, (size_t)alignment);
 }
 
 extern "C" int64_t s2attn_diff_backward_workspace_bytes(const s2attn_shape *shape)
@@ -3452,10 +3531,10 @@ extern "C" int s2attn_diff_backward(const void *k, const void *v, const void *q,
     a.dy = dy, a.ysaved = y, a.y2saved = y2, a.lse2 = reinterpret_cast<float2 *>(const_cast<float *>(lse)), a.dq = dq, a.dk = dk, a.dv = dv, a.dlam = dlam;
     a.dstats = static_cast<float4 *>(workspace);
     a.lam_part = reinterpret_cast<float *>(a.dstats + stat_points(shape));
-    a.lam_n = shape->nlat_out * shape->nlon_out;
-    rc = launch_diff(DQ, a, shape->dtype, static_cast<hipStream_t>(stream));
+    const int family = diff_family(a, shape->dtype, common_alignment({k, v, q, dy, y, y2, dk, dv, dq}));
+    rc = launch_diff(DQ, family, a, shape->dtype, static_cast<hipStream_t>(stream));
     if (rc != S2ATTN_OK || (!dk && !dlam)) return rc;
-    return launch_diff(DKDV, a, shape->dtype, static_cast<hipStream_t>(stream));
+    return launch_diff(DKDV, family, a, shape->dtype, static_cast<hipStream_t>(stream));
 }
 
 namespace {
