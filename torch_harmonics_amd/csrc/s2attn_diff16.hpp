@@ -78,22 +78,25 @@ template <typename M, int D, bool PAD> struct DiffOwn {
             for (int s = 0; s < NS; s++)
                 if (has(i, s)) settle(op[i][s]);
     }
-    // does block s hold channels of map i?  (PAD: perhaps)
-    static constexpr __device__ bool has(int i, int s) { return PAD || D == 32 || (i == 0 ? s < NS / 2 : s >= NS / 2); }
+    // Does block s hold channels of map i?  PAD: it may, for some d.  (Decided when compiled: a branch on d around matrix instructions saves a few
+    // of them, but the compiler, which waits for their results where it reads them, does not count right over the edges of such
+    // branches: reads after too few clocks, seen in its output and in results.)
+    static constexpr __device__ bool has(int i, int s) { return i == 0 ? 2 * s < (NS > 1 ? NS : 2) : PAD || D == 32 || 2 * s >= NS; }
     // sc[i] += (16 staged rows) x own, both maps
-    __device__ inline void scores(f4v &s0, f4v &s1, const char *blk, int c, int qd, int d) const
+    __device__ inline void scores(f4v &s0, f4v &s1, const char *blk, int c, int qd) const
     {
 #pragma unroll
         for (int s = 0; s < NS; s++) {
             const uint4 x = h16_read_row<DiffBand<D>::PITCH>(blk, s, c, qd);
-            if (has(0, s) && (!PAD || 32 * s < d)) s0 = M::mfma(x, op[0][s], s0);
-            if (has(1, s) && (!PAD || (32 * s + 32 > d && 32 * s < 2 * d))) s1 = M::mfma(x, op[1][s], s1);
+            if (has(0, s)) s0 = M::mfma(x, op[0][s], s0);
+            if (has(1, s)) s1 = M::mfma(x, op[1][s], s1);
         }
     }
 };
 
-// Sums over positions of row[channel] * coefficient for rows of two maps: 16-channel block cb takes the coefficients of its map.  Where a block holds
-// channels of both (PAD with d an odd multiple of 8) it is computed with either, the second in `both`.
+// Sums over positions of row[channel] * coefficient for rows of two maps: 16-channel block cb takes the coefficients of its map (PAD: chosen by
+// selects, not by branches, see DiffOwn::has).  The block that channel d lies in may hold channels of both: it is computed with either, the
+// second map's in `both`.
 template <typename M, int D, bool PAD> struct DiffSum {
     static constexpr int NCB = D / 16;
     f4v acc[NCB], both;
@@ -103,17 +106,16 @@ template <typename M, int D, bool PAD> struct DiffSum {
         for (int cb = 0; cb < NCB; cb++) acc[cb] = f4v{0.f, 0.f, 0.f, 0.f};
         both = f4v{0.f, 0.f, 0.f, 0.f};
     }
-    __device__ inline void add(int cb, uint4 rows, uint4 p0, uint4 p1, int d)
+    static __device__ inline uint4 of_map(int cb, uint4 p0, uint4 p1, int d)
     {
-        if (!PAD) {
-            acc[cb] = M::mfma(rows, cb < NCB / 2 ? p0 : p1, acc[cb]);
-        } else if (16 * cb < d) {
-            acc[cb] = M::mfma(rows, p0, acc[cb]);
-            if (16 * cb + 16 > d) both = M::mfma(rows, p1, both);
-        } else if (16 * cb < 2 * d) {
-            acc[cb] = M::mfma(rows, p1, acc[cb]);
-        }
+        if (NCB > 1 && cb >= NCB / 2) return p1;
+        if (!PAD || cb == 0) return p0;
+        const bool first = 16 * cb < d;
+        return make_uint4(first ? p0.x : p1.x, first ? p0.y : p1.y, first ? p0.z : p1.z, first ? p0.w : p1.w);
     }
+    __device__ inline void add(int cb, uint4 rows, uint4 p0, uint4 p1, int d) { acc[cb] = M::mfma(rows, of_map(cb, p0, p1, d), acc[cb]); }
+    // PAD: rows of the 16-channel block d / 16
+    __device__ inline void add_both(uint4 rows, uint4 p1) { both = M::mfma(rows, p1, both); }
     // of this lane's channels 16 cb + 4 qd .. + 4
     __device__ inline f4v value(int cb, int qd, int d) const { return PAD && 16 * cb < d && 16 * cb + 4 * qd >= d ? both : acc[cb]; }
     static __device__ inline bool first(int cb, int qd, int d) { return PAD ? 16 * cb + 4 * qd < d : cb < NCB / 2; }
@@ -226,7 +228,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
                 sc[0][kb] = sc[1][kb] = f4v{0.f, 0.f, 0.f, 0.f};
-                own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd, d);
+                own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd);
             }
             const int tb = pos + 4 * qd - c; // neighbor index of element (kb, v): tb + 16 kb + v
             if (!(pos >= HQ - 1 && pos + HK <= len)) {
@@ -402,7 +404,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 sc[0][kb] = f4v{l0, l0, l0, l0};
                 sc[1][kb] = f4v{l1, l1, l1, l1};
                 gc[kb] = f4v{-D1, -D1, -D1, -D1};
-                own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd, d);
+                own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd);
 #pragma unroll
                 for (int s = 0; s < NS; s++) gc[kb] = M::mfma(h16_read_row<PITCH>(vblk[kb], s, c, qd), gop[s], gc[kb]);
             }
@@ -427,6 +429,11 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 const uint4 kt = h16_read_transposed<PITCH>(kblk[0], kblk[1], cb, c, qd);
                 acc.add(cb, kt, d0, d1, d);
                 ak.add(cb, kt, p0, p1, d);
+            }
+            if (PAD) {
+                const uint4 kt = h16_read_transposed<PITCH>(kblk[0], kblk[1], d / 16, c, qd);
+                acc.add_both(kt, d1);
+                ak.add_both(kt, p1);
             }
         }
         if (wk.more) {
@@ -580,7 +587,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 sc[1][qb] = *reinterpret_cast<const f4v *>(sq + 16);
                 gc[qb] = *reinterpret_cast<const f4v *>(sg);
                 step[qb] = *reinterpret_cast<const f4v *>(sg + 16);
-                own.scores(sc[0][qb], sc[1][qb], qblk[qb], c, qd, d);
+                own.scores(sc[0][qb], sc[1][qb], qblk[qb], c, qd);
 #pragma unroll
                 for (int s = 0; s < NS; s++) gc[qb] = M::mfma(h16_read_row<PITCH>(gblk[qb], s, c, qd), vop[s], gc[qb]);
             }
@@ -603,6 +610,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 dvt[cb] = M::mfma(h16_read_transposed<PITCH>(gblk[0], gblk[1], cb, c, qd), cop, dvt[cb]);
                 dkt.add(cb, h16_read_transposed<PITCH>(qblk[0], qblk[1], cb, c, qd), d0, d1, d);
             }
+            if (PAD) dkt.add_both(h16_read_transposed<PITCH>(qblk[0], qblk[1], d / 16, c, qd), d1);
         }
         if (wk.more) {
             if (wk.fresh) __syncthreads(); // the next run's rows replace rows the slowest wavefront may still be reading

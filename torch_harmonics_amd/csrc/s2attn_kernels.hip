@@ -36,11 +36,12 @@
 
 #include "s2attn_internal.h"
 
-// This file is compiled eight times (see the Makefile), so that the groups of kernel instantiations build side by
+// This file is compiled nine times (see the Makefile), so that the groups of kernel instantiations build side by
 // side: S2_PART 1 = everything but the launchers of the 16-longitude matrix-core families, 2 = the 16-bit family
 // (s2attn_h16.hpp), 3 = the fp32 family (s2attn_m32.hpp), 4 = its ring-step kernels for 16-bit storage, 5 = the split-product family
 // (s2attn_s16.hpp), 6 = its ring steps
-// (s2attn_s16_ring.hpp), 7 = differential attention one point at a time (s2attn_diff.hpp), 8 = in 16-bit tiles (s2attn_diff16.hpp).  S2_PART 0 (the default) is the whole library in one unit.
+// (s2attn_s16_ring.hpp), 7 = differential attention one point at a time (s2attn_diff.hpp), 8 = in 16-bit tiles (s2attn_diff16.hpp), 9 = on
+// split products (s2attn_diffsplit.hpp).  S2_PART 0 (the default) is the whole library in one unit.
 #ifndef S2_PART
 #define S2_PART 0
 #endif
@@ -2285,6 +2286,7 @@ template <typename T> __global__ __launch_bounds__(64) void dkdv_mfma_kernel(con
 #include "s2attn_s16_ring.hpp"
 #include "s2attn_diff.hpp"
 #include "s2attn_diff16.hpp"
+#include "s2attn_diffsplit.hpp"
 
 // ---------------------------------------------------------------------------------
 // layout permutes: batched 2-D transpose [R, S] -> [S, R] through a 64x65 LDS tile
@@ -2325,6 +2327,7 @@ template <int D, int MODE, typename T> int launch_ring_m32(const Args &a0, hipSt
 template <int D, bool WRITE, typename T> int launch_ring_pass2_m32(const Args &a0, hipStream_t stream);
 template <typename T> int launch_diff_points(Which which, const DArgs &a, hipStream_t stream);
 template <typename T, int D, bool PAD> int launch_d16(Which which, const DArgs &a, hipStream_t stream);
+template <typename T, int D, bool PAD> int launch_dsplit(Which which, const DArgs &a, hipStream_t stream);
 
 #if S2_PART == 0 || S2_PART == 2
 // 16-bit matrix-core kernels: bf16 / fp16 storage, head dim D, equal longitude counts, 16-byte aligned tensors.  The
@@ -2624,6 +2627,28 @@ template <typename T, int D, bool PAD> int launch_d16(Which which, const DArgs &
 S2_D16_INSTANCES(bf16_t)
 S2_D16_INSTANCES(f16_t)
 #undef S2_D16_INSTANCES
+#endif
+#if S2_PART == 0 || S2_PART == 9
+template <typename T, int D, bool PAD> int launch_dsplit(Which which, const DArgs &a, hipStream_t stream)
+{
+    void (*const kern)(const DArgs) = which == FWD ? fwd_dsplit_kernel<T, D, PAD> : which == DQ ? dq_dsplit_kernel<T, D, PAD> : dkdv_dsplit_kernel<T, D, PAD>;
+    return launch_diff_tiles(kern, which, a, dsplit_lds_bytes<T, D>(which == DKDV), stream);
+}
+#endif
+#if S2_PART == 9
+template int launch_dsplit<float, 16, false>(Which, const DArgs &, hipStream_t);
+template int launch_dsplit<float, 32, false>(Which, const DArgs &, hipStream_t);
+template int launch_dsplit<float, 64, false>(Which, const DArgs &, hipStream_t);
+template int launch_dsplit<float, 128, false>(Which, const DArgs &, hipStream_t);
+template int launch_dsplit<float, 128, true>(Which, const DArgs &, hipStream_t);
+#define S2_DSPLIT_INSTANCES(T)                                                 \
+    template int launch_dsplit<T, 16, true>(Which, const DArgs &, hipStream_t); \
+    template int launch_dsplit<T, 32, true>(Which, const DArgs &, hipStream_t); \
+    template int launch_dsplit<T, 64, true>(Which, const DArgs &, hipStream_t);
+S2_DSPLIT_INSTANCES(float)
+S2_DSPLIT_INSTANCES(bf16_t)
+S2_DSPLIT_INSTANCES(f16_t)
+#undef S2_DSPLIT_INSTANCES
 #endif
 } // namespace s2
 
@@ -3453,6 +3478,8 @@ template <typename T> int diff_family_t(const DArgs &a, size_t alignment)
         const bool strides = (a.ldk | a.ldv | a.ldq | a.ldy | a.ldg | a.lddk | a.lddv | a.lddq) % 8 == 0;
         if (a.dk_ % 16 == 0 && a.dv_ % 8 == 0 && c <= 128 && strides && alignment % 16 == 0) return S2ATTN_FAMILY_16BIT;
     }
+    const bool fp32 = std::is_same<T, float>::value;
+    if (a.dk_ % 8 == 0 && a.dv_ % 4 == 0 && c <= (fp32 ? 128 : 64) && alignment % (fp32 ? 4 : 8) == 0) return S2ATTN_FAMILY_SPLIT;
     return S2ATTN_FAMILY_VECTOR;
 }
 int diff_family(const DArgs &a, int dtype, size_t alignment)
@@ -3478,6 +3505,18 @@ template <typename T> int launch_diff_t(Which which, int family, DArgs &a, hipSt
             if (c <= 64) return exact && c == 64 ? launch_d16<T, 64, false>(which, a, stream) : launch_d16<T, 64, true>(which, a, stream);
             return exact && c == 128 ? launch_d16<T, 128, false>(which, a, stream) : launch_d16<T, 128, true>(which, a, stream);
         }
+    }
+    if (family == S2ATTN_FAMILY_SPLIT) {
+        const int c = std::max(a.dk_, a.dv_);
+        if constexpr (std::is_same<T, float>::value) {
+            const bool exact = a.dk_ == a.dv_;
+            if (exact && c == 16) return launch_dsplit<T, 16, false>(which, a, stream);
+            if (exact && c == 32) return launch_dsplit<T, 32, false>(which, a, stream);
+            if (exact && c == 64) return launch_dsplit<T, 64, false>(which, a, stream);
+            if (c > 64) return exact && c == 128 ? launch_dsplit<T, 128, false>(which, a, stream) : launch_dsplit<T, 128, true>(which, a, stream);
+        }
+        if (c <= 16) return launch_dsplit<T, 16, true>(which, a, stream);
+        return c <= 32 ? launch_dsplit<T, 32, true>(which, a, stream) : launch_dsplit<T, 64, true>(which, a, stream);
     }
     return launch_diff_points<T>(which, a, stream);
 }
