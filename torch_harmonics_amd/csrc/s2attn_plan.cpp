@@ -21,7 +21,8 @@ struct HostRun {
 };
 
 // One CSR row -> maximal runs of consecutive columns inside one latitude of the OTHER grid (nlon columns per latitude);
-// a run that ends at nlon - 1 is joined with a run of the same latitude that starts at 0 into one circular run.
+// a run that ends at nlon - 1 is joined with a run of the same latitude that starts at 0 into one circular run, whichever of
+// the two the row lists first (ascending columns list 0 first, an arc from its west end on lists it last).
 struct RawRun {
     int32_t lat, ws, len;
 };
@@ -47,6 +48,9 @@ int row_runs(const int64_t *col_idx, int64_t z0, int64_t z1, int nlat, int nlon,
         if (j > i && row[i].ws == 0 && row[j].ws + row[j].len == nlon && row[i].len + row[j].len <= nlon) {
             row[j].len += row[i].len;
             row[i].len = 0; // dropped
+        } else if (j > i && row[j].ws == 0 && row[i].ws + row[i].len == nlon && row[i].len + row[j].len <= nlon) {
+            row[i].len += row[j].len;
+            row[j].len = 0;
         }
         i = j + 1;
     }
