@@ -58,14 +58,12 @@ template <int D> constexpr int d16_lds_bytes() { return 2 * DiffBand<D>::BYTES; 
 template <typename M, int D, bool PAD> struct DiffOwn {
     static constexpr int NS = D / 32;
     uint4 op[2][NS];
-    template <bool SCALED> __device__ inline void load(const char *row, int qd, int d)
+    __device__ inline void load(const char *row, int qd, int d)
     {
 #pragma unroll
         for (int s = 0; s < NS; s++) {
             const int ch = 32 * s + 8 * qd;
-            uint4 x = h16_load_piece(row + 2 * ch, !PAD || ch < 2 * d);
-            if (SCALED) x = h16_scale_log2e<M>(x);
-            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            const uint4 x = h16_load_piece(row + 2 * ch, !PAD || ch < 2 * d), zero = make_uint4(0u, 0u, 0u, 0u);
             op[0][s] = ch < d ? x : zero;
             op[1][s] = ch < d ? zero : x;
         }
@@ -178,7 +176,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     const size_t pt = (size_t)query_point(a, b, ho, ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
 
     DiffOwn<M, D, PAD> own;
-    own.template load<false>(static_cast<const char *>(a.q) + (pt * a.ldq + (size_t)h * nk) * 2, qd, d);
+    own.load(static_cast<const char *>(a.q) + (pt * a.ldq + (size_t)h * nk) * 2, qd, d);
     f4v acc[2][NCB], Z[2]; // Y^T of each map: register v of block cb is channel 16 cb + 4 qd + v of column c; sums of probabilities
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -331,8 +329,8 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     const size_t sidx = ((size_t)bh * a.Ho + ho) * a.Wo + w0 + (mine ? c : 0);
     const float lam = load_as_f32(a.lam, h, a.lam_dtype);
 
-    DiffOwn<M, D, PAD> own; // q log2 e
-    own.template load<true>(static_cast<const char *>(a.q) + (pt * a.ldq + (size_t)h * nk) * 2, qd, d);
+    DiffOwn<M, D, PAD> own;
+    own.load(static_cast<const char *>(a.q) + (pt * a.ldq + (size_t)h * nk) * 2, qd, d);
     uint4 gop[NS];
     float D1 = 0.f, D2 = 0.f;
 #pragma unroll
@@ -397,12 +395,12 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
             const int xw = HQ * wave + pos; // band row of this wavefront's position `pos`
             const char *kblk[2] = {band_block<PITCH>(Ks, xw), band_block<PITCH>(Ks, xw + 16)};
             const char *vblk[2] = {band_block<PITCH>(Vs, xw), band_block<PITCH>(Vs, xw + 16)};
-            // The accumulators start at log2 w - lse and at -D1, so the matrix cores hand back the exponents of p and g - D1.
+            // g starts at -D1, so the matrix cores hand back g - D1.  (The scores could start at log2 w - lse with log2 e in q's operand: rounding
+            // that to 16 bits again moves a score of s by s 2^-9, and so every p alike: half of the error of the gradients, and no faster.)
             f4v sc[2][2], gc[2];
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
-                sc[0][kb] = f4v{l0, l0, l0, l0};
-                sc[1][kb] = f4v{l1, l1, l1, l1};
+                sc[0][kb] = sc[1][kb] = f4v{0.f, 0.f, 0.f, 0.f};
                 gc[kb] = f4v{-D1, -D1, -D1, -D1};
                 own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd);
 #pragma unroll
@@ -416,8 +414,8 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
                     const bool in = inner || (unsigned)(tb + 16 * kb + v) < (unsigned)len;
-                    sc[0][kb][v] = in ? fast_exp2(sc[0][kb][v]) : 0.f;
-                    sc[1][kb][v] = in ? fast_exp2(sc[1][kb][v]) : 0.f;
+                    sc[0][kb][v] = in ? fast_exp2(fmaf(sc[0][kb][v], LOG2E, l0)) : 0.f;
+                    sc[1][kb][v] = in ? fast_exp2(fmaf(sc[1][kb][v], LOG2E, l1)) : 0.f;
                     ds[0][kb][v] = sc[0][kb][v] * gc[kb][v];
                     ds[1][kb][v] = sc[1][kb][v] * (gc[kb][v] + step21);
                 }
@@ -482,7 +480,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 // ---- backward, dk/dv pass: transposed gather (see dkdv_h16_kernel) -------------------------------------------------------------------
 // Per step and map S = Q K^T; G = dY V^T once; dV^T += dY^T (P1 - lam P2) once; dK^T += Q^T dS.
 // The statistics of the staged queries lie in the padding of the rings' rows 4 j: log2 w - lse of the two maps for rows 4 j .. + 4 in that of Q, -D1
-// and D1 - D2 in that of dY, so a lane reads them as start values of its accumulators.
+// and D1 - D2 in that of dY, so a lane reads those of its four queries at once.
 template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void dkdv_d16_kernel(const DArgs a)
 {
     typedef DiffBand<D> Tile;
@@ -508,8 +506,8 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     const size_t pt = (size_t)key_point(a, b, hi, hi / a.kps) + (size_t)(w0 + (mine ? c : 0)) * a.kps;
     float lam = load_as_f32(a.lam, h, a.lam_dtype);
 
-    DiffOwn<M, D, PAD> own; // k log2 e
-    own.template load<true>(static_cast<const char *>(a.k) + (pt * a.ldk + (size_t)h * nk) * 2, qd, d);
+    DiffOwn<M, D, PAD> own;
+    own.load(static_cast<const char *>(a.k) + (pt * a.ldk + (size_t)h * nk) * 2, qd, d);
     uint4 vop[NS];
 #pragma unroll
     for (int s = 0; s < NS; s++) vop[s] = h16_load_piece(static_cast<const char *>(a.v) + (pt * a.ldv + (size_t)h * nv) * 2 + 16 * qd + 64 * s, !PAD || 32 * s + 8 * qd < nv);
@@ -579,12 +577,13 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
             const int xw = HQ * wave + pos; // band row of this wavefront's position `pos`
             const char *qblk[2] = {band_block<PITCH>(Qs, xw), band_block<PITCH>(Qs, xw + 16)};
             const char *gblk[2] = {band_block<PITCH>(Gs, xw), band_block<PITCH>(Gs, xw + 16)};
-            f4v sc[2][2], gc[2], step[2];
+            f4v sc[2][2], gc[2], l0[2], l1[2], step[2];
 #pragma unroll
             for (int qb = 0; qb < 2; qb++) {
                 const char *sq = qblk[qb] + 4 * qd * PITCH + STAT, *sg = gblk[qb] + 4 * qd * PITCH + STAT;
-                sc[0][qb] = *reinterpret_cast<const f4v *>(sq);
-                sc[1][qb] = *reinterpret_cast<const f4v *>(sq + 16);
+                sc[0][qb] = sc[1][qb] = f4v{0.f, 0.f, 0.f, 0.f};
+                l0[qb] = *reinterpret_cast<const f4v *>(sq);
+                l1[qb] = *reinterpret_cast<const f4v *>(sq + 16);
                 gc[qb] = *reinterpret_cast<const f4v *>(sg);
                 step[qb] = *reinterpret_cast<const f4v *>(sg + 16);
                 own.scores(sc[0][qb], sc[1][qb], qblk[qb], c, qd);
@@ -599,7 +598,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
                     const bool in = inner || (unsigned)(tb + 16 * qb + v) < (unsigned)len;
-                    const float p0 = in ? fast_exp2(sc[0][qb][v]) : 0.f, p1 = in ? fast_exp2(sc[1][qb][v]) : 0.f;
+                    const float p0 = in ? fast_exp2(fmaf(sc[0][qb][v], LOG2E, l0[qb][v])) : 0.f, p1 = in ? fast_exp2(fmaf(sc[1][qb][v], LOG2E, l1[qb][v])) : 0.f;
                     co[qb][v] = fmaf(-lam, p1, p0);
                     ds[0][qb][v] = p0 * gc[qb][v];
                     ds[1][qb][v] = p1 * (gc[qb][v] + step[qb][v]);
