@@ -105,6 +105,8 @@ int s2attn_abi_version(void);
  *     gather_span [2*nvout]   per virtual output latitude (first column, columns): an arc of the circle that holds every
  *                 neighbor column of query column 0 (of query column j: the arc shifted by j); columns = the whole
  *                 circle when the runs do not fit a shorter arc
+ *     quads       per grouping the groups of four latitudes that the differential kernels work on, in launch order, and the
+ *                 bands of the other grid that a group's latitudes see (s2attn_plan.cpp, build_quads)
  * The builder runs on the host; the caller copies the blob to the device unchanged (it can also be stored and reused:
  * it depends only on the CSR and the four grid extents) and passes the device address with a host copy of the header.
  *
@@ -141,6 +143,7 @@ enum {
     S2ATTN_PH_SCATTER_PAIR_RUNS = 24,
     S2ATTN_PH_SCATTER_NPAIRS = 25,
     S2ATTN_PH_GATHER_SPAN = 26, /* nvout x (first column, columns): an arc holding every neighbor column of query column 0 */
+    S2ATTN_PH_QUADS = 27, /* 0: none (virtual latitudes of 16128 columns or more) */
     S2ATTN_PH_NLAT_IN = 28, /* the grid extents the plan was built for: checked against the shape of every call */
     S2ATTN_PH_NLON_IN = 29,
     S2ATTN_PH_NLAT_OUT = 30,

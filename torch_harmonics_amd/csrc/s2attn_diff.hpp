@@ -9,6 +9,11 @@
 // The forward keeps y2 and the two normalisers (log2 Zi) for the backward.  A point that sees nothing (no neighbor, or only latitudes of weight
 // zero) has y = 0 and its normalisers are +inf, so that all its probabilities are zero in the backward.
 
+// n / d for 0 <= n < 2^24, 0 < d < 2^24: m = floor(2^s / d) + 1, s = 24 + ceil(log2 d): n m / 2^s is less than 1 / d too large
+struct QuadDiv {
+    unsigned m;
+    int s;
+};
 struct DArgs : Args {
     const void *lam; // [nh], of type lam_dtype
     void *dlam;      // [nh], of type lam_dtype, or null
@@ -19,6 +24,10 @@ struct DArgs : Args {
     float *lam_part; // [B * nh][lam_n] summands of -dlam, written by the dq pass
     int lam_n;
     int lam_dtype;
+    // the plan's bands of four latitudes (s2attn_plan.cpp, build_quads) in the pass's grouping; quads: the section
+    const int *quads, *q_list, *q_bands;
+    int q_groups;
+    QuadDiv q_first, q_tiles, q_head;
     int lam_blocks;  // leading workgroups of the dk/dv launch that sum dlam, a head each
 };
 

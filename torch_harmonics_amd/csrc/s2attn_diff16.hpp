@@ -1,8 +1,7 @@
 // Differential attention on 16-bit matrix instructions, 16-bit storage.  Included by s2attn_kernels.hip inside namespace s2 after s2attn_diff.hpp.
 //
-// Tiling, staging and the layout of scores as in s2attn_h16.hpp: a workgroup of four wavefronts owns 64 consecutive longitudes of one
-// latitude, 16 per wavefront, and walks its runs in steps of 32 band positions on one staged band of k and v (q and dy); lane l = (c = l %
-// 16, qd = l / 16); scores are produced transposed, S^T[position][column].
+// Tiles as in s2attn_quads.hpp: sixteen columns of a latitude per wavefront, steps of 32 band positions; lane l = (c = l % 16, qd = l / 16);
+// scores are produced transposed, S^T[position][column].  Facts about the instruction as in s2attn_h16.hpp.
 //
 // The row of k (q) holds both maps' channels and is staged once; map i's scores take the 32-channel blocks it has channels in, with the other map's
 // channels zero on the side that stays in registers.  <dy, v>, the masks, the staged rows and the transposed reads of v serve both maps.
@@ -12,47 +11,36 @@
 // Shape domain: ck a multiple of 8, cv a multiple of 8, 2 ck and cv at most D (a tile is D channels wide, 32, 64 or 128; zeros are staged past
 // a head's channels and never stored; PAD = false: 2 ck = cv = D), at least 32 columns per virtual latitude, rows 16-byte aligned.
 
-template <int D> struct DiffBand {
-    static constexpr int CPR = D / 8;                   // 16-byte pieces per row
-    static constexpr int PITCH = 2 * D + 32;            // bytes (32 or 96 modulo 128: free of bank conflicts, see WgBand)
-    static constexpr int RPI = 64 * NW / CPR;           // rows per iteration of the workgroup
-    static constexpr int NIT = (FRESH + RPI - 1) / RPI; // iterations for the first step of a run
-    static constexpr int BYTES = BR * PITCH;            // one tensor's ring
-    u4v ra[NIT], rb[NIT];
+template <int D, bool PAD> struct DiffStage {
+    typedef QuadPieces<D / 8> P;
+    static constexpr int PITCH = 2 * D + 32;    // bytes (32 or 96 modulo 128: free of bank conflicts, see WgBand)
+    static constexpr int BYTES = 2 * HK * PITCH; // one buffer
+    uint4 r[P::N];
+    float4 st; // dk/dv pass: the statistics of row tid
+    float w;   // gather: the quadrature weight
 
-    // N rows from longitude cs on (0 <= cs < W); lda, ldb: bytes between two columns; a_ok, b_ok: this thread's piece lies in the row
-    template <int N, bool PAD> __device__ inline void fetch(const char *pa, const char *pb, int tid, int cs, int W, unsigned lda, unsigned ldb, bool a_ok, bool b_ok)
+    // rows cs .. cs + n of W columns; lda, ldb: bytes between two columns; na, nb channels.  (Rows past n stay an earlier step's.)
+    __device__ inline void fetch(const char *pa, const char *pb, int tid, int cs, int W, int n, unsigned lda, unsigned ldb, int na, int nb)
     {
-        const int r0 = tid / CPR;
-        const unsigned pc = 16u * (tid % CPR);
 #pragma unroll
-        for (int it = 0; it < (N + RPI - 1) / RPI; it++) {
-            if (PAD) ra[it] = u4v{0u, 0u, 0u, 0u}, rb[it] = u4v{0u, 0u, 0u, 0u};
-            if ((it + 1) * RPI <= N || it * RPI + r0 < N) {
-                unsigned col = (unsigned)(cs + r0); // r0 < RPI <= 64 <= 2 W
-                col = min(col, col - (unsigned)W);  // col - W wraps to a huge value when col < W
-                if (RPI > 32) col = min(col, col - (unsigned)W);
-                if (!PAD || a_ok) ra[it] = *reinterpret_cast<const u4v *>(pa + col * lda + pc);
-                if (!PAD || b_ok) rb[it] = *reinterpret_cast<const u4v *>(pb + col * ldb + pc);
-            }
-            cs += RPI;
-            while (cs >= W) cs -= W;
+        for (int it = 0; it < P::N; it++) {
+            const int i = P::at(it, tid);
+            const bool second = P::second(i);
+            unsigned col = (unsigned)(cs + P::row(i));
+            col = min(col, col - (unsigned)W); // (wraps to a huge value when col < W; 32 <= W)
+            if (P::row(i) < n) r[it] = h16_load_piece((second ? pb : pa) + col * (second ? ldb : lda) + 16 * P::piece(i), !PAD || 8 * P::piece(i) < (second ? nb : na));
         }
     }
-    template <int N> __device__ inline void commit(char *A, char *B, int tid, int x0) const
+    __device__ inline void commit(char *buf, int tid) const
     {
-        const int r0 = tid / CPR, pc = 16 * (tid % CPR);
 #pragma unroll
-        for (int it = 0; it < (N + RPI - 1) / RPI; it++) {
-            if ((it + 1) * RPI <= N || it * RPI + r0 < N) {
-                const int o = ((x0 + it * RPI + r0) & (BR - 1)) * PITCH + pc;
-                *reinterpret_cast<u4v *>(A + o) = ra[it];
-                *reinterpret_cast<u4v *>(B + o) = rb[it];
-            }
+        for (int it = 0; it < P::N; it++) {
+            const int i = P::at(it, tid);
+            if (P::on(i)) *reinterpret_cast<uint4 *>(buf + (P::second(i) ? HK * PITCH : 0) + P::row(i) * PITCH + 16 * P::piece(i)) = r[it];
         }
     }
 };
-template <int D> constexpr int d16_lds_bytes() { return 2 * DiffBand<D>::BYTES; }
+template <int D> constexpr int d16_lds_bytes(bool stats) { return 2 * (DiffStage<D, false>::BYTES + (stats ? HK * 16 : 0)); }
 
 // The lane's own row of both maps (a query's q, or a key's k): op[i][s] = channels 32 s + 8 qd .. + 8 of its row that belong to map i, zeros elsewhere
 template <typename M, int D, bool PAD> struct DiffOwn {
@@ -85,7 +73,7 @@ template <typename M, int D, bool PAD> struct DiffOwn {
     {
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            const uint4 x = h16_read_row<DiffBand<D>::PITCH>(blk, s, c, qd);
+            const uint4 x = h16_read_row<DiffStage<D, PAD>::PITCH>(blk, s, c, qd);
             if (has(0, s)) s0 = M::mfma(x, op[0][s], s0);
             if (has(1, s)) s1 = M::mfma(x, op[1][s], s1);
         }
@@ -146,34 +134,35 @@ template <typename T, int D, Which PASS> __device__ __forceinline__ void diff_re
 {
     __threadfence(); // what is written here comes after it
     const DArgs a = diff_point_args();
-    S2_H16_IDS_OF(64 * wv + point_lane(), block, PASS == DKDV ? a.Wi : a.Wo, PASS == DKDV ? a.Hi : a.Ho)
-    (void)c, (void)qd, (void)nvalid;
-    const int row = (PASS == DKDV ? a.sorder : a.gorder)[rowsel];
+    const QuadUnit u = quad_unit(a, block);
+    const int lane = point_lane(), row = QUAD * u.g + wv;
     for (; redo; redo &= redo - 1) {
-        const int col = w0 + __builtin_ctz(redo);
-        if (PASS == FWD) diff_point_forward<T, D / 16>(a, b, h, bh, row, col, lane);
-        if (PASS == DQ) diff_point_dq<T, D / 16>(a, b, h, bh, row, col, lane);
-        if (PASS == DKDV) diff_point_dkdv<T, D / 16>(a, b, h, bh, row, col, lane);
+        const int col = u.w0 + __builtin_ctz(redo);
+        if (PASS == FWD) diff_point_forward<T, D / 16>(a, u.b, u.h, u.bh, row, col, lane);
+        if (PASS == DQ) diff_point_dq<T, D / 16>(a, u.b, u.h, u.bh, row, col, lane);
+        if (PASS == DKDV) diff_point_dkdv<T, D / 16>(a, u.b, u.h, u.bh, row, col, lane);
     }
 }
+
+// Registers decide how many wavefronts a SIMD holds; where the compiler comes close to one more by itself, the launch bounds ask for it (dk/dv pass, 64
+// channels, 361x720: 143 registers and three 379 us, 128 and four 326).
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
 template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void fwd_d16_kernel(const DArgs a)
 {
-    typedef DiffBand<D> Tile;
+    typedef DiffStage<D, PAD> Tile;
     typedef H16<T> M;
     constexpr int PITCH = Tile::PITCH, NCB = D / 16;
     extern __shared__ __attribute__((aligned(16))) char h16_lds[];
-    char *Ks = h16_lds, *Vs = h16_lds + Tile::BYTES;
-
-    S2_H16_IDS(a.Wo, a.Ho)
-    const int wv = __builtin_amdgcn_readfirstlane(wave);
-    const int ho = a.gorder[rowsel];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, qd = lane >> 4, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const QuadUnit u = quad_unit(a, blockIdx.x);
+    const int bh = u.bh, b = u.b, h = u.h, w0 = u.w0;
+    const int ho = min(QUAD * u.g + wv, a.Ho - 1); // (a latitude that is not there sees nothing and stores nothing)
     const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
     const char *kx = static_cast<const char *>(a.k) + ((size_t)b * a.Hi * a.Wi * a.ldk + (size_t)h * nk) * 2;
     const char *vx = static_cast<const char *>(a.v) + ((size_t)b * a.Hi * a.Wi * a.ldv + (size_t)h * nv) * 2;
-    const bool mine = c < nvalid;
-    const size_t pt = (size_t)query_point(a, b, ho, ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
+    const bool mine = QUAD * u.g + wv < a.Ho && w0 + c < a.Wo;
+    const size_t pt = (size_t)query_point(a, b, ho, a.qps == 1 ? ho : ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
 
     DiffOwn<M, D, PAD> own;
     own.load(static_cast<const char *>(a.q) + (pt * a.ldq + (size_t)h * nk) * 2, qd, d);
@@ -187,54 +176,45 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     float m[2] = {NEG_BIG, NEG_BIG};
     const uint4 ones = d16_ones<M>();
 
-    H16Walk wk;
-    wk.ri = a.goff[ho];
-    wk.rend = a.goff[ho + 1];
-    wk.pos = 0;
-    wk.run = Run{0, 0, 0, 0};
-    Tile bd;
+    QuadWalk wk;
+    Tile bd = {}; // the next step's rows, on their way
     const unsigned lda = 2u * a.ldk * a.kps, ldb = 2u * a.ldv * a.kps; // bytes between two columns of a virtual input latitude
-    const bool a_ok = 8 * (tid % Tile::CPR) < nk, b_ok = 8 * (tid % Tile::CPR) < nv;
-    auto fetch = [&](const Run &rn, bool fresh) {
-        const size_t row = (size_t)key_row(a, rn.lat, rn.pad);
-        const int cs = wk.stage(fresh, rn.ws + wg0, a.Wi);
-        if (fresh)
-            bd.template fetch<FRESH, PAD>(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, cs, a.Wi, lda, ldb, a_ok, b_ok);
-        else
-            bd.template fetch<HK, PAD>(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, cs, a.Wi, lda, ldb, a_ok, b_ok);
+    auto fetch = [&]() {
+        const size_t row = quad_row(wk.lat, wk.aux, a.kps, a.Wi);
+        bd.w = a.quad_w[wk.aux + wk.zero];
+        bd.fetch(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, wk.column(w0, a.Wi), a.Wi, wk.rows(), lda, ldb, nk, nv);
     };
-    wk.w = 1.f;
-    if (wk.ri < wk.rend) {
-        wk.run = a.gruns[wk.ri];
-        wk.w = a.quad_w[wk.run.pad];
-        fetch(wk.run, true);
-        bd.template commit<FRESH>(Ks, Vs, tid, 0);
+    char *buf = h16_lds, *other = h16_lds + Tile::BYTES;
+    wk.start(a, u, wv, lane);
+    QuadStep cur = wk.step();
+    float weight = 1.f;
+    if (cur.some) {
+        fetch();
+        bd.commit(buf, tid);
+        weight = bd.w;
     }
     __syncthreads();
     own.settle_();
 
-    while (wk.ri < wk.rend) {
-        wk.plan(a.gruns, a.quad_w);
-        if (wk.more) fetch(wk.nrun, wk.fresh);
-        if (active) {
-            const float lw = fast_log2(wk.w);
-            const int len = wk.run.len, pos = wk.pos;
-            const int xw = HQ * wave + pos; // band row of this wavefront's position `pos`
-            const char *kblk[2] = {band_block<PITCH>(Ks, xw), band_block<PITCH>(Ks, xw + 16)};
-            const char *vblk[2] = {band_block<PITCH>(Vs, xw), band_block<PITCH>(Vs, xw + 16)};
+    while (cur.some) {
+        wk.follow();
+        fetch();
+        if (cur.seen()) {
+            const float lw = fast_log2(weight);
+            const char *kblk[2] = {buf, buf + 16 * PITCH}, *vblk[2] = {buf + HK * PITCH, buf + (HK + 16) * PITCH};
             f4v sc[2][2]; // [map][block]
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
                 sc[0][kb] = sc[1][kb] = f4v{0.f, 0.f, 0.f, 0.f};
                 own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd);
             }
-            const int tb = pos + 4 * qd - c; // neighbor index of element (kb, v): tb + 16 kb + v
-            if (!(pos >= HQ - 1 && pos + HK <= len)) {
+            const int tb = cur.pos - cur.d + 4 * qd - c; // neighbor index of element (kb, v): tb + 16 kb + v
+            if (!cur.inner()) {
 #pragma unroll
                 for (int kb = 0; kb < 2; kb++)
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
-                        const bool in = (unsigned)(tb + 16 * kb + v) < (unsigned)len;
+                        const bool in = (unsigned)(tb + 16 * kb + v) < (unsigned)cur.l;
                         sc[0][kb][v] = in ? sc[0][kb][v] : -INFINITY;
                         sc[1][kb][v] = in ? sc[1][kb][v] : -INFINITY;
                     }
@@ -274,16 +254,12 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 acc[1][cb] = M::mfma(vt, p[1], acc[1][cb]);
             }
         }
-        if (wk.more) {
-            if (wk.fresh) {
-                __syncthreads(); // the next run's rows replace rows the slowest wavefront may still be reading
-                bd.template commit<FRESH>(Ks, Vs, tid, 0);
-            } else {
-                bd.template commit<HK>(Ks, Vs, tid, FRESH - HK + wk.npos);
-            }
-        }
+        bd.commit(other, tid);
+        weight = bd.w;
         __syncthreads();
-        wk.advance();
+        char *t = buf;
+        buf = other, other = t;
+        cur = wk.step();
     }
 
     float check = Z[0][0] + Z[1][0];
@@ -310,22 +286,21 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 
 // ---- backward, dq pass -----------------------------------------------------------------------------------------------------------
 // Per step and map S^T = K Q^T; G^T = V dY^T once; dQ^T += K^T dS^T, and AK^T += K^T P^T and sum dS for the corrections of D.
-template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void dq_d16_kernel(const DArgs a)
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <= 64 && !PAD ? 4 : 1) void dq_d16_kernel(const DArgs a)
 {
-    typedef DiffBand<D> Tile;
+    typedef DiffStage<D, PAD> Tile;
     typedef H16<T> M;
     constexpr int PITCH = Tile::PITCH, NS = D / 32, NCB = D / 16;
     extern __shared__ __attribute__((aligned(16))) char h16_lds[];
-    char *Ks = h16_lds, *Vs = h16_lds + Tile::BYTES;
-
-    S2_H16_IDS(a.Wo, a.Ho)
-    const int wv = __builtin_amdgcn_readfirstlane(wave);
-    const int ho = a.gorder[rowsel];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, qd = lane >> 4, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const QuadUnit u = quad_unit(a, blockIdx.x);
+    const int bh = u.bh, b = u.b, h = u.h, w0 = u.w0;
+    const int ho = min(QUAD * u.g + wv, a.Ho - 1); // (a latitude that is not there sees nothing and stores nothing)
     const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
     const char *kx = static_cast<const char *>(a.k) + ((size_t)b * a.Hi * a.Wi * a.ldk + (size_t)h * nk) * 2;
     const char *vx = static_cast<const char *>(a.v) + ((size_t)b * a.Hi * a.Wi * a.ldv + (size_t)h * nv) * 2;
-    const bool mine = c < nvalid;
-    const size_t pt = (size_t)query_point(a, b, ho, ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
+    const bool mine = QUAD * u.g + wv < a.Ho && w0 + c < a.Wo;
+    const size_t pt = (size_t)query_point(a, b, ho, a.qps == 1 ? ho : ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
     const size_t sidx = ((size_t)bh * a.Ho + ho) * a.Wo + w0 + (mine ? c : 0);
     const float lam = load_as_f32(a.lam, h, a.lam_dtype);
 
@@ -357,28 +332,22 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     f4v off[2] = {f4v{0.f, 0.f, 0.f, 0.f}, f4v{0.f, 0.f, 0.f, 0.f}};
     const uint4 ones = d16_ones<M>();
 
-    H16Walk wk;
-    wk.ri = a.goff[ho];
-    wk.rend = a.goff[ho + 1];
-    wk.pos = 0;
-    wk.run = Run{0, 0, 0, 0};
-    Tile bd;
-    const unsigned lda = 2u * a.ldk * a.kps, ldb = 2u * a.ldv * a.kps;
-    const bool a_ok = 8 * (tid % Tile::CPR) < nk, b_ok = 8 * (tid % Tile::CPR) < nv;
-    auto fetch = [&](const Run &rn, bool fresh) {
-        const size_t row = (size_t)key_row(a, rn.lat, rn.pad);
-        const int cs = wk.stage(fresh, rn.ws + wg0, a.Wi);
-        if (fresh)
-            bd.template fetch<FRESH, PAD>(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, cs, a.Wi, lda, ldb, a_ok, b_ok);
-        else
-            bd.template fetch<HK, PAD>(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, cs, a.Wi, lda, ldb, a_ok, b_ok);
+    QuadWalk wk;
+    Tile bd = {}; // the next step's rows, on their way
+    const unsigned lda = 2u * a.ldk * a.kps, ldb = 2u * a.ldv * a.kps; // bytes between two columns of a virtual input latitude
+    auto fetch = [&]() {
+        const size_t row = quad_row(wk.lat, wk.aux, a.kps, a.Wi);
+        bd.w = a.quad_w[wk.aux + wk.zero];
+        bd.fetch(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, wk.column(w0, a.Wi), a.Wi, wk.rows(), lda, ldb, nk, nv);
     };
-    wk.w = 1.f;
-    if (wk.ri < wk.rend) {
-        wk.run = a.gruns[wk.ri];
-        wk.w = a.quad_w[wk.run.pad];
-        fetch(wk.run, true);
-        bd.template commit<FRESH>(Ks, Vs, tid, 0);
+    char *buf = h16_lds, *other = h16_lds + Tile::BYTES;
+    wk.start(a, u, wv, lane);
+    QuadStep cur = wk.step();
+    float weight = 1.f;
+    if (cur.some) {
+        fetch();
+        bd.commit(buf, tid);
+        weight = bd.w;
     }
     __syncthreads();
     own.settle_();
@@ -386,15 +355,12 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     settle(lse.x), settle(lse.y);
     const float step21 = D1 - D2; // g - D2 = (g - D1) + (D1 - D2)
 
-    while (wk.ri < wk.rend) {
-        wk.plan(a.gruns, a.quad_w);
-        if (wk.more) fetch(wk.nrun, wk.fresh);
-        if (active) {
-            const float lw = fast_log2(wk.w), l0 = lw - lse.x, l1 = lw - lse.y;
-            const int len = wk.run.len, pos = wk.pos;
-            const int xw = HQ * wave + pos; // band row of this wavefront's position `pos`
-            const char *kblk[2] = {band_block<PITCH>(Ks, xw), band_block<PITCH>(Ks, xw + 16)};
-            const char *vblk[2] = {band_block<PITCH>(Vs, xw), band_block<PITCH>(Vs, xw + 16)};
+    while (cur.some) {
+        wk.follow();
+        fetch();
+        if (cur.seen()) {
+            const float lw = fast_log2(weight), l0 = lw - lse.x, l1 = lw - lse.y;
+            const char *kblk[2] = {buf, buf + 16 * PITCH}, *vblk[2] = {buf + HK * PITCH, buf + (HK + 16) * PITCH};
             // g starts at -D1, so the matrix cores hand back g - D1.  (The scores could start at log2 w - lse with log2 e in q's operand: rounding
             // that to 16 bits again moves a score of s by s 2^-9, and so every p alike: half of the error of the gradients, and no faster.)
             f4v sc[2][2], gc[2];
@@ -406,14 +372,14 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 #pragma unroll
                 for (int s = 0; s < NS; s++) gc[kb] = M::mfma(h16_read_row<PITCH>(vblk[kb], s, c, qd), gop[s], gc[kb]);
             }
-            const int tb = pos + 4 * qd - c;
-            const bool inner = pos >= HQ - 1 && pos + HK <= len; // every element of the step is a neighbor: no band mask
+            const int tb = cur.pos - cur.d + 4 * qd - c;
+            const bool inner = cur.inner(); // every element of the step is a neighbor: no band mask
             f4v ds[2][2];
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
-                    const bool in = inner || (unsigned)(tb + 16 * kb + v) < (unsigned)len;
+                    const bool in = inner || (unsigned)(tb + 16 * kb + v) < (unsigned)cur.l;
                     sc[0][kb][v] = in ? fast_exp2(fmaf(sc[0][kb][v], LOG2E, l0)) : 0.f;
                     sc[1][kb][v] = in ? fast_exp2(fmaf(sc[1][kb][v], LOG2E, l1)) : 0.f;
                     ds[0][kb][v] = sc[0][kb][v] * gc[kb][v];
@@ -434,16 +400,12 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 ak.add_both(kt, p1);
             }
         }
-        if (wk.more) {
-            if (wk.fresh) {
-                __syncthreads(); // the next run's rows replace rows the slowest wavefront may still be reading
-                bd.template commit<FRESH>(Ks, Vs, tid, 0);
-            } else {
-                bd.template commit<HK>(Ks, Vs, tid, FRESH - HK + wk.npos);
-            }
-        }
+        bd.commit(other, tid);
+        weight = bd.w;
         __syncthreads();
-        wk.advance();
+        char *t = buf;
+        buf = other, other = t;
+        cur = wk.step();
     }
 
     // (stored after the walk: a global store ahead of the loop would turn the loop's scalar loads of runs and weights,
@@ -470,7 +432,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 *reinterpret_cast<uint2 *>(dq + 32 * cb) = make_uint2(M::pack2(x[0], x[1]), M::pack2(x[2], x[3]));
             }
     }
-    if (active) {
+    if (QUAD * u.g + wv < a.Ho) {
         part = point_lanes_sum(part);
         if (lane == 0) a.lam_part[(size_t)bh * a.lam_n + (size_t)ho * ((a.Wo + HQ - 1) / HQ) + w0 / HQ] = part;
     }
@@ -479,31 +441,30 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 
 // ---- backward, dk/dv pass: transposed gather (see dkdv_h16_kernel) -------------------------------------------------------------------
 // Per step and map S = Q K^T; G = dY V^T once; dV^T += dY^T (P1 - lam P2) once; dK^T += Q^T dS.
-// The statistics of the staged queries lie in the padding of the rings' rows 4 j: log2 w - lse of the two maps for rows 4 j .. + 4 in that of Q, -D1
-// and D1 - D2 in that of dY, so a lane reads those of its four queries at once.
-template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void dkdv_d16_kernel(const DArgs a)
+// The statistics of the staged queries lie behind the buffers, log2 w - lse of the two maps, -D1 and D1 - D2, each for 32 rows, so a lane reads
+// those of its four queries at once.  (The key's log2 w is added to the first two in 32 bits.)
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <= 32 ? 5 : D <= 64 ? 4 : 1) void dkdv_d16_kernel(const DArgs a)
 {
-    typedef DiffBand<D> Tile;
+    typedef DiffStage<D, PAD> Tile;
     typedef H16<T> M;
     constexpr int PITCH = Tile::PITCH, NS = D / 32, NCB = D / 16;
     extern __shared__ __attribute__((aligned(16))) char h16_lds[];
-    char *Qs = h16_lds, *Gs = h16_lds + Tile::BYTES;
-    constexpr int STAT = 2 * D;
     if ((int)blockIdx.x < a.lam_blocks) {
         diff_sum_lam(a, blockIdx.x, threadIdx.x, 64 * NW, reinterpret_cast<double *>(h16_lds));
         return;
     }
     const int block = blockIdx.x - a.lam_blocks;
 
-    S2_H16_IDS_OF(threadIdx.x, block, a.Wi, a.Hi)
-    const int wv = __builtin_amdgcn_readfirstlane(wave);
-    const int hi = a.sorder[rowsel];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, qd = lane >> 4, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const QuadUnit u = quad_unit(a, block);
+    const int bh = u.bh, b = u.b, h = u.h, w0 = u.w0;
+    const int hi = min(QUAD * u.g + wv, a.Hi - 1);
     const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
     const char *qy = static_cast<const char *>(a.q) + ((size_t)b * a.Ho * a.Wo * a.ldq + (size_t)h * nk) * 2;
     const char *gy = static_cast<const char *>(a.dy) + ((size_t)b * a.Ho * a.Wo * a.ldg + (size_t)h * nv) * 2;
     const float4 *stats = a.dstats + (size_t)bh * a.Ho * a.Wo;
-    const bool mine = c < nvalid;
-    const size_t pt = (size_t)key_point(a, b, hi, hi / a.kps) + (size_t)(w0 + (mine ? c : 0)) * a.kps;
+    const bool mine = QUAD * u.g + wv < a.Hi && w0 + c < a.Wi;
+    const size_t pt = (size_t)key_point(a, b, hi, a.kps == 1 ? hi : hi / a.kps) + (size_t)(w0 + (mine ? c : 0)) * a.kps;
     float lam = load_as_f32(a.lam, h, a.lam_dtype);
 
     DiffOwn<M, D, PAD> own;
@@ -516,92 +477,68 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     f4v dvt[NCB];
 #pragma unroll
     for (int cb = 0; cb < NCB; cb++) dvt[cb] = f4v{0.f, 0.f, 0.f, 0.f};
-    const float lw = fast_log2(a.quad_w[hi / a.kps]);
+    const float lw = fast_log2(a.quad_w[a.kps == 1 ? hi : hi / a.kps]);
 
-    H16Walk wk;
-    wk.ri = a.soff[hi];
-    wk.rend = a.soff[hi + 1];
-    wk.pos = 0;
-    wk.run = Run{0, 0, 0, 0};
-    wk.w = 1.f;
-    Tile bd;
-    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+    QuadWalk wk;
+    Tile bd = {}; // the next step's rows, on their way
     const unsigned lda = 2u * a.ldq * a.qps, ldb = 2u * a.ldg * a.qps; // bytes between two columns of a virtual output latitude
-    const bool a_ok = 8 * (tid % Tile::CPR) < nk, b_ok = 8 * (tid % Tile::CPR) < nv;
-    auto fetch = [&](const Run &rn, bool fresh) {
-        int c0 = 0;
-        if (fresh) { // longitude of band row 0, in [0, 2 W)
-            c0 = wg0 - rn.ws - rn.len + 1 + a.Wo;
-            while (c0 < 0) c0 += a.Wo;
-        }
-        const int cs = wk.stage(fresh, c0, a.Wo);
-        const size_t row = (size_t)query_row(a, rn.lat, rn.pad);
-        if (fresh)
-            bd.template fetch<FRESH, PAD>(qy + 2 * row * a.ldq, gy + 2 * row * a.ldg, tid, cs, a.Wo, lda, ldb, a_ok, b_ok);
-        else
-            bd.template fetch<HK, PAD>(qy + 2 * row * a.ldq, gy + 2 * row * a.ldg, tid, cs, a.Wo, lda, ldb, a_ok, b_ok);
-        if (tid < (fresh ? FRESH : HK)) { // the first threads fetch the statistics of the staged rows
-            int col = cs + tid;
-            while (col >= a.Wo) col -= a.Wo;
-            st = stats[(size_t)rn.lat * a.Wo + col];
+    auto fetch = [&]() {
+        const size_t row = quad_row(wk.lat, wk.aux, a.qps, a.Wo);
+        const int cs = wk.column(w0, a.Wo), n = wk.rows();
+        bd.fetch(qy + 2 * row * a.ldq, gy + 2 * row * a.ldg, tid, cs, a.Wo, n, lda, ldb, nk, nv);
+        int col = cs + min(tid & (HK - 1), n - 1); // (the first threads' are used)
+        if (col >= a.Wo) col -= a.Wo;
+        bd.st = stats[(size_t)wk.lat * a.Wo + col];
+    };
+    auto commit = [&](char *to) {
+        bd.commit(to, tid);
+        if (tid < HK) {
+            float *t = reinterpret_cast<float *>(to + Tile::BYTES) + tid;
+            t[0] = -bd.st.x, t[HK] = -bd.st.y, t[2 * HK] = -bd.st.z, t[3 * HK] = bd.st.z - bd.st.w;
         }
     };
-    auto commit = [&](int x0) {
-        if (x0 == 0)
-            bd.template commit<FRESH>(Qs, Gs, tid, 0);
-        else
-            bd.template commit<HK>(Qs, Gs, tid, x0);
-        if (tid < (x0 == 0 ? FRESH : HK)) {
-            const int o = ((x0 + tid) & (BR - 4)) * PITCH + STAT + 4 * (tid & 3);
-            *reinterpret_cast<float *>(Qs + o) = lw - st.x;
-            *reinterpret_cast<float *>(Qs + o + 16) = lw - st.y;
-            *reinterpret_cast<float *>(Gs + o) = -st.z;
-            *reinterpret_cast<float *>(Gs + o + 16) = st.z - st.w;
-        }
-    };
-    if (wk.ri < wk.rend) {
-        wk.run = a.sruns[wk.ri];
-        fetch(wk.run, true);
-        commit(0);
+    char *buf = h16_lds, *other = h16_lds + Tile::BYTES + HK * 16;
+    wk.start(a, u, wv, lane);
+    QuadStep cur = wk.step();
+    if (cur.some) {
+        fetch();
+        commit(buf);
     }
     __syncthreads();
     own.settle_();
     settle(vop);
     settle(lam);
 
-    while (wk.ri < wk.rend) {
-        wk.plan(a.sruns);
-        if (wk.more) fetch(wk.nrun, wk.fresh);
-        if (active) {
-            const int len = wk.run.len, pos = wk.pos;
-            const int xw = HQ * wave + pos; // band row of this wavefront's position `pos`
-            const char *qblk[2] = {band_block<PITCH>(Qs, xw), band_block<PITCH>(Qs, xw + 16)};
-            const char *gblk[2] = {band_block<PITCH>(Gs, xw), band_block<PITCH>(Gs, xw + 16)};
-            f4v sc[2][2], gc[2], l0[2], l1[2], step[2];
+    while (cur.some) {
+        wk.follow();
+        fetch();
+        if (cur.seen()) {
+            const char *qblk[2] = {buf, buf + 16 * PITCH}, *gblk[2] = {buf + HK * PITCH, buf + (HK + 16) * PITCH};
+            const float *stat = reinterpret_cast<const float *>(buf + Tile::BYTES) + 4 * qd;
+            f4v sc[2][2], gc[2], l0[2], l1[2], step21[2];
 #pragma unroll
             for (int qb = 0; qb < 2; qb++) {
-                const char *sq = qblk[qb] + 4 * qd * PITCH + STAT, *sg = gblk[qb] + 4 * qd * PITCH + STAT;
                 sc[0][qb] = sc[1][qb] = f4v{0.f, 0.f, 0.f, 0.f};
-                l0[qb] = *reinterpret_cast<const f4v *>(sq);
-                l1[qb] = *reinterpret_cast<const f4v *>(sq + 16);
-                gc[qb] = *reinterpret_cast<const f4v *>(sg);
-                step[qb] = *reinterpret_cast<const f4v *>(sg + 16);
+                l0[qb] = *reinterpret_cast<const f4v *>(stat + 16 * qb) + lw;
+                l1[qb] = *reinterpret_cast<const f4v *>(stat + 16 * qb + HK) + lw;
+                gc[qb] = *reinterpret_cast<const f4v *>(stat + 16 * qb + 2 * HK);
+                step21[qb] = *reinterpret_cast<const f4v *>(stat + 16 * qb + 3 * HK);
                 own.scores(sc[0][qb], sc[1][qb], qblk[qb], c, qd);
 #pragma unroll
                 for (int s = 0; s < NS; s++) gc[qb] = M::mfma(h16_read_row<PITCH>(gblk[qb], s, c, qd), vop[s], gc[qb]);
             }
-            const int tb = pos + 4 * qd - c; // r - c of element (qb, v): tb + 16 qb + v
-            const bool inner = pos >= HQ - 1 && pos + HK <= len; // every element of the step is a (query, key) pair of the run
+            const int tb = cur.pos - cur.d + 4 * qd - c; // r - c of element (qb, v): tb + 16 qb + v
+            const bool inner = cur.inner(); // every element of the step is a (query, key) pair of the band
             f4v ds[2][2], co[2];
 #pragma unroll
             for (int qb = 0; qb < 2; qb++)
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
-                    const bool in = inner || (unsigned)(tb + 16 * qb + v) < (unsigned)len;
+                    const bool in = inner || (unsigned)(tb + 16 * qb + v) < (unsigned)cur.l;
                     const float p0 = in ? fast_exp2(fmaf(sc[0][qb][v], LOG2E, l0[qb][v])) : 0.f, p1 = in ? fast_exp2(fmaf(sc[1][qb][v], LOG2E, l1[qb][v])) : 0.f;
                     co[qb][v] = fmaf(-lam, p1, p0);
                     ds[0][qb][v] = p0 * gc[qb][v];
-                    ds[1][qb][v] = p1 * (gc[qb][v] + step[qb][v]);
+                    ds[1][qb][v] = p1 * (gc[qb][v] + step21[qb][v]);
                 }
             const uint4 cop = d16_pack<M>(co), d0 = d16_pack<M>(ds[0]), d1 = d16_pack<M>(ds[1]);
 #pragma unroll
@@ -611,12 +548,11 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
             }
             if (PAD) dkt.add_both(h16_read_transposed<PITCH>(qblk[0], qblk[1], d / 16, c, qd), d1);
         }
-        if (wk.more) {
-            if (wk.fresh) __syncthreads(); // the next run's rows replace rows the slowest wavefront may still be reading
-            commit(wk.fresh ? 0 : FRESH - HK + wk.npos);
-        }
+        commit(other);
         __syncthreads();
-        wk.advance();
+        char *t = buf;
+        buf = other, other = t;
+        cur = wk.step();
     }
 
     float check = 0.f;

@@ -1,8 +1,9 @@
 // Differential attention with the accuracy of fp32 on bf16 matrix instructions, for fp32 storage and for 16-bit head widths that the kernels of
 // s2attn_diff16.hpp do not take.  Included by s2attn_kernels.hip inside namespace s2 after s2attn_diff16.hpp.
 //
-// Tiling and layout as there, values as terms as in s2attn_s16.hpp: staged rows are split once per workgroup, probabilities and dS once per
-// step, and a product is the six term products of at most second order.
+// Tiles and layout as there, values as terms as in s2attn_s16.hpp: staged rows are split once per workgroup, probabilities and dS once per
+// step, and a product is the six term products of at most second order.  A step's products are added to sums of 32 bits, those of low order first; the
+// forward and the dk/dv pass keep one register per sum, not two, and so a wavefront more per SIMD (181x360, 4 x 64 channels, forward: 281 -> 249 us).
 //
 // Shape domain: ck and cv multiples of 4, 2 ck and cv at most D (16, 32, 64; fp32 also 128), at least 32 columns per virtual latitude, rows
 // aligned to four 16-bit values, or to a float.
@@ -135,70 +136,116 @@ template <typename A, int D, int S, bool PAD> struct SplitMapSum {
     }
 };
 
-template <typename T, int D> constexpr int dsplit_lds_bytes(bool stats) { return 2 * SplitBand<T, D, false>::BYTES + (stats ? FRESH * 16 : 0); }
+// The rows of a step: a piece of eight channels per thread and iteration, split as it goes to LDS
+template <typename T, int D, bool PAD> struct SplitStage {
+    typedef QuadPieces<D / 8> P;
+    static constexpr int S = S16Piece<T>::S, PITCH = s16_pitch<D, S>(), BYTES = 2 * HK * PITCH;
+    S16Piece<T> r[P::N];
+    float w; // gather: the quadrature weight
+
+    // rows cs .. cs + n of W columns; columns lda, ldb elements apart; na, nb channels
+    __device__ inline void fetch(const T *pa, const T *pb, int tid, int cs, int W, int n, unsigned lda, unsigned ldb, int na, int nb)
+    {
+#pragma unroll
+        for (int it = 0; it < P::N; it++) {
+            const int i = P::at(it, tid);
+            const bool second = P::second(i);
+            unsigned col = (unsigned)(cs + min(P::row(i), n - 1));
+            col = min(col, col - (unsigned)W); // (wraps to a huge value when col < W; 32 <= W)
+            r[it].template load<PAD>((second ? pb : pa) + col * (second ? ldb : lda), 8 * P::piece(i), second ? nb : na);
+        }
+    }
+    // SCALED: the first tensor's times log2 e (fp32)
+    template <bool SCALED = false> __device__ inline void commit(char *buf, int tid)
+    {
+#pragma unroll
+        for (int it = 0; it < P::N; it++) {
+            const int i = P::at(it, tid);
+            if constexpr (SCALED) {
+                const float f = P::second(i) ? 1.f : LOG2E;
+                r[it].a *= f, r[it].b *= f;
+            }
+            uint4 t[3];
+            s16_terms<T>(t, r[it]);
+            if (P::on(i)) {
+                char *o = buf + (P::second(i) ? HK * PITCH : 0) + P::row(i) * PITCH + 16 * P::piece(i);
+#pragma unroll
+                for (int k = 0; k < S; k++) *reinterpret_cast<uint4 *>(o + 2 * D * k) = t[k];
+            }
+        }
+    }
+};
+template <typename T, int D> constexpr int dsplit_lds_bytes(bool stats) { return 2 * (SplitStage<T, D, false>::BYTES + (stats ? HK * 16 : 0)); }
+
+// Start values of a step's scores: `start` where the point sees the position
+__device__ inline void quad_start(S16Sum (&sc)[2], const QuadStep &cur, int tb, float start)
+{
+    sc[0].lo = sc[1].lo = f4v{0.f, 0.f, 0.f, 0.f};
+    sc[0].hi = sc[1].hi = f4v{start, start, start, start};
+    if (!cur.inner()) {
+        tb += cur.pos - cur.d;
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) sc[kb].hi[v] = (unsigned)(tb + 16 * kb + v) < (unsigned)cur.l ? start : -INFINITY;
+    }
+}
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
-template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void fwd_dsplit_kernel(const DArgs a)
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <= 32 ? 4 : 1) void fwd_dsplit_kernel(const DArgs a)
 {
-    typedef SplitBand<T, D, PAD> Band_;
+    typedef SplitStage<T, D, PAD> Band_;
     constexpr int S = Band_::S, PITCH = Band_::PITCH, NCB = D / 16;
     extern __shared__ __attribute__((aligned(16))) char h16_lds[];
-    char *Ks = h16_lds, *Vs = h16_lds + Band_::BYTES;
-
-    S2_H16_IDS(a.Wo, a.Ho)
-    const int wv = __builtin_amdgcn_readfirstlane(wave);
-    const int ho = a.gorder[rowsel];
-    const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, qd = lane >> 4, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const QuadUnit u = quad_unit(a, blockIdx.x);
+    const int bh = u.bh, b = u.b, h = u.h, w0 = u.w0;
+    const int ho = min(QUAD * u.g + wv, a.Ho - 1); // (a latitude that is not there sees nothing and stores nothing)
+    const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D;
     const T *kx = static_cast<const T *>(a.k) + (size_t)b * a.Hi * a.Wi * a.ldk + h * nk;
     const T *vx = static_cast<const T *>(a.v) + (size_t)b * a.Hi * a.Wi * a.ldv + h * nv;
-    const bool mine = c < nvalid;
-    const size_t pt = (size_t)query_point(a, b, ho, ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
+    const bool mine = QUAD * u.g + wv < a.Ho && w0 + c < a.Wo;
+    const size_t pt = (size_t)query_point(a, b, ho, a.qps == 1 ? ho : ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
 
     SplitMaps<T, D, true, PAD> own; // q log2 e: scores come out in the log2 domain
     own.load(static_cast<const T *>(a.q) + pt * a.ldq + h * nk, nk, qd);
-    S16Sum acc[2][NCB];
+    typedef SplitMapSum<f4v, D, S, PAD> Sums;
+    f4v acc[2][NCB];
     s16_zero(acc[0]), s16_zero(acc[1]);
     float m[2] = {0.f, 0.f}, Z[2] = {0.f, 0.f};
     bool first = true; // this column has seen no neighbor of positive weight
 
-    H16Walk wk;
-    wk.ri = a.goff[ho];
-    wk.rend = a.goff[ho + 1];
-    wk.pos = 0;
-    wk.run = Run{0, 0, 0, 0};
+    QuadWalk wk;
     Band_ bd;
     const unsigned lda = a.ldk * a.kps, ldb = a.ldv * a.kps; // elements between two columns of a virtual input latitude
-    auto fetch = [&](const Run &rn, bool fresh) {
-        const size_t row = (size_t)key_row(a, rn.lat, rn.pad);
-        const int cs = wk.stage(fresh, rn.ws + wg0, a.Wi);
-        if (fresh)
-            bd.template fetch<FRESH>(kx + row * a.ldk, vx + row * a.ldv, tid, cs, a.Wi, lda, ldb, nk, nv);
-        else
-            bd.template fetch<HK>(kx + row * a.ldk, vx + row * a.ldv, tid, cs, a.Wi, lda, ldb, nk, nv);
+    auto fetch = [&]() {
+        const size_t row = quad_row(wk.lat, wk.aux, a.kps, a.Wi);
+        bd.w = a.quad_w[wk.aux + wk.zero];
+        bd.fetch(kx + row * a.ldk, vx + row * a.ldv, tid, wk.column(w0, a.Wi), a.Wi, wk.rows(), lda, ldb, nk, nv);
     };
-    wk.w = 1.f;
-    if (wk.ri < wk.rend) {
-        wk.run = a.gruns[wk.ri];
-        wk.w = a.quad_w[wk.run.pad];
-        fetch(wk.run, true);
-        bd.template commit<FRESH>(Ks, Vs, tid, 0);
+    char *buf = h16_lds, *other = h16_lds + Band_::BYTES;
+    wk.start(a, u, wv, lane);
+    QuadStep cur = wk.step();
+    float weight = 1.f;
+    if (cur.some) {
+        fetch();
+        bd.commit(buf, tid);
+        weight = bd.w;
     }
     __syncthreads();
     own.settle_();
 
     const int tb = 4 * qd - c;
-    int rb = 0; // ring block of band position `pos`
-    while (wk.ri < wk.rend) {
-        wk.plan(a.gruns, a.quad_w);
-        if (wk.more) fetch(wk.nrun, wk.fresh);
-        if (active) {
-            const int b0 = s16_block(rb, wv), b1 = s16_block(b0, 1);
-            const char *k0 = Ks + b0 * 16 * PITCH, *k1 = Ks + b1 * 16 * PITCH, *v0 = Vs + b0 * 16 * PITCH, *v1 = Vs + b1 * 16 * PITCH;
+    while (cur.some) {
+        wk.follow();
+        fetch();
+        if (cur.seen()) {
+            const char *k0 = buf, *k1 = buf + 16 * PITCH, *v0 = buf + HK * PITCH, *v1 = buf + (HK + 16) * PITCH;
             // The sums start at log2 w - m, so they end as the exponents of the probabilities.
             S16Sum s0[2], s1[2];
-            const float lw = fast_log2(wk.w);
-            s16_start(s0, tb, wk.pos, wk.run.len, lw - m[0]);
-            s16_start(s1, tb, wk.pos, wk.run.len, lw - m[1]);
+            const float lw = fast_log2(weight);
+            quad_start(s0, cur, tb, lw - m[0]);
+            quad_start(s1, cur, tb, lw - m[1]);
             own.scores(s0[0], s1[0], k0, c, qd);
             own.scores(s0[1], s1[1], k1, c, qd);
             f4v p[2][2] = {{s16_value(s0[0]), s16_value(s0[1])}, {s16_value(s1[0]), s16_value(s1[1])}};
@@ -216,7 +263,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                     const float corr = first ? 0.f : fast_exp2(-dm);
                     Z[i] *= corr;
 #pragma unroll
-                    for (int cb = 0; cb < NCB; cb++) acc[i][cb].hi *= corr, acc[i][cb].lo *= corr;
+                    for (int cb = 0; cb < NCB; cb++) acc[i][cb] *= corr;
                     p[i][0] -= dm, p[i][1] -= dm;
                     m[i] += dm;
                     seen |= cm > -INFINITY;
@@ -240,26 +287,22 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 uint4 x[3];
 #pragma unroll
                 for (int n = 0; n < S; n++) x[n] = h16_read_transposed<PITCH>(v0 + 2 * D * n, v1 + 2 * D * n, cb, c, qd);
-                s16_mma<S, 3>(acc[0][cb], x, ps[0]);
-                s16_mma<S, 3>(acc[1][cb], x, ps[1]);
+                Sums::mma(acc[0][cb], x, ps[0]);
+                Sums::mma(acc[1][cb], x, ps[1]);
             }
         }
-        if (wk.more) {
-            __syncthreads(); // the next rows replace rows the slowest wavefront may still be reading
-            rb = wk.fresh ? 0 : s16_block(rb, 2);
-            if (wk.fresh)
-                bd.template commit<FRESH>(Ks, Vs, tid, 0);
-            else
-                bd.template commit<HK>(Ks, Vs, tid, 16 * s16_block(rb, 3));
-        }
+        bd.commit(other, tid);
+        weight = bd.w;
         __syncthreads();
-        wk.advance();
+        char *t = buf;
+        buf = other, other = t;
+        cur = wk.step();
     }
 
     const float z0 = h16_quarter_sum(Z[0]), z1 = h16_quarter_sum(Z[1]);
     float check = z0 + z1;
 #pragma unroll
-    for (int cb = 0; cb < NCB; cb++) check += point_sum(s16_value(acc[0][cb]) + s16_value(acc[1][cb]));
+    for (int cb = 0; cb < NCB; cb++) check += point_sum(acc[0][cb] + acc[1][cb]);
     const unsigned redo = point_columns(mine && not_finite(check));
     if (mine) {
         if (a.lse2 && qd == 0)
@@ -270,8 +313,8 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 #pragma unroll
         for (int cb = 0; cb < NCB; cb++)
             if (!PAD || 16 * cb + 4 * qd < nv) {
-                const f4v o2 = s16_value(acc[1][cb]) * i1;
-                s16_store4(y + 16 * cb, s16_value(acc[0][cb]) * i0 - lam * o2);
+                const f4v o2 = acc[1][cb] * i1;
+                s16_store4(y + 16 * cb, acc[0][cb] * i0 - lam * o2);
                 if (a.y2) s16_store4(y2 + 16 * cb, o2);
             }
     }
@@ -281,19 +324,18 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 // ---- backward, dq pass -----------------------------------------------------------------------------------------------------------
 template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void dq_dsplit_kernel(const DArgs a)
 {
-    typedef SplitBand<T, D, PAD> Band_;
+    typedef SplitStage<T, D, PAD> Band_;
     constexpr int S = Band_::S, PITCH = Band_::PITCH, NCB = D / 16;
     extern __shared__ __attribute__((aligned(16))) char h16_lds[];
-    char *Ks = h16_lds, *Vs = h16_lds + Band_::BYTES;
-
-    S2_H16_IDS(a.Wo, a.Ho)
-    const int wv = __builtin_amdgcn_readfirstlane(wave);
-    const int ho = a.gorder[rowsel];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, qd = lane >> 4, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const QuadUnit u = quad_unit(a, blockIdx.x);
+    const int bh = u.bh, b = u.b, h = u.h, w0 = u.w0;
+    const int ho = min(QUAD * u.g + wv, a.Ho - 1); // (a latitude that is not there sees nothing and stores nothing)
     const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
     const T *kx = static_cast<const T *>(a.k) + (size_t)b * a.Hi * a.Wi * a.ldk + h * nk;
     const T *vx = static_cast<const T *>(a.v) + (size_t)b * a.Hi * a.Wi * a.ldv + h * nv;
-    const bool mine = c < nvalid;
-    const size_t pt = (size_t)query_point(a, b, ho, ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
+    const bool mine = QUAD * u.g + wv < a.Ho && w0 + c < a.Wo;
+    const size_t pt = (size_t)query_point(a, b, ho, a.qps == 1 ? ho : ho / a.qps) + (size_t)(w0 + (mine ? c : 0)) * a.qps;
     const size_t sidx = ((size_t)bh * a.Ho + ho) * a.Wo + w0 + (mine ? c : 0);
     const float lam = load_as_f32(a.lam, h, a.lam_dtype);
 
@@ -328,27 +370,22 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     ak.zero();
     float off[2] = {0.f, 0.f};
 
-    H16Walk wk;
-    wk.ri = a.goff[ho];
-    wk.rend = a.goff[ho + 1];
-    wk.pos = 0;
-    wk.run = Run{0, 0, 0, 0};
+    QuadWalk wk;
     Band_ bd;
-    const unsigned lda = a.ldk * a.kps, ldb = a.ldv * a.kps;
-    auto fetch = [&](const Run &rn, bool fresh) {
-        const size_t row = (size_t)key_row(a, rn.lat, rn.pad);
-        const int cs = wk.stage(fresh, rn.ws + wg0, a.Wi);
-        if (fresh)
-            bd.template fetch<FRESH>(kx + row * a.ldk, vx + row * a.ldv, tid, cs, a.Wi, lda, ldb, nk, nv);
-        else
-            bd.template fetch<HK>(kx + row * a.ldk, vx + row * a.ldv, tid, cs, a.Wi, lda, ldb, nk, nv);
+    const unsigned lda = a.ldk * a.kps, ldb = a.ldv * a.kps; // elements between two columns of a virtual input latitude
+    auto fetch = [&]() {
+        const size_t row = quad_row(wk.lat, wk.aux, a.kps, a.Wi);
+        bd.w = a.quad_w[wk.aux + wk.zero];
+        bd.fetch(kx + row * a.ldk, vx + row * a.ldv, tid, wk.column(w0, a.Wi), a.Wi, wk.rows(), lda, ldb, nk, nv);
     };
-    wk.w = 1.f;
-    if (wk.ri < wk.rend) {
-        wk.run = a.gruns[wk.ri];
-        wk.w = a.quad_w[wk.run.pad];
-        fetch(wk.run, true);
-        bd.template commit<FRESH>(Ks, Vs, tid, 0);
+    char *buf = h16_lds, *other = h16_lds + Band_::BYTES;
+    wk.start(a, u, wv, lane);
+    QuadStep cur = wk.step();
+    float weight = 1.f;
+    if (cur.some) {
+        fetch();
+        bd.commit(buf, tid);
+        weight = bd.w;
     }
     __syncthreads();
     qo.settle_();
@@ -357,18 +394,16 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     const float step21 = D1 - D2; // g - D2 = (g - D1) + (D1 - D2)
 
     const int tb = 4 * qd - c;
-    int rb = 0;
-    while (wk.ri < wk.rend) {
-        wk.plan(a.gruns, a.quad_w);
-        if (wk.more) fetch(wk.nrun, wk.fresh);
-        if (active) {
-            const int b0 = s16_block(rb, wv), b1 = s16_block(b0, 1);
-            const char *k0 = Ks + b0 * 16 * PITCH, *k1 = Ks + b1 * 16 * PITCH, *v0 = Vs + b0 * 16 * PITCH, *v1 = Vs + b1 * 16 * PITCH;
+    while (cur.some) {
+        wk.follow();
+        fetch();
+        if (cur.seen()) {
+            const char *k0 = buf, *k1 = buf + 16 * PITCH, *v0 = buf + HK * PITCH, *v1 = buf + (HK + 16) * PITCH;
             // The sums start at log2 w - lse and at -D1, so they end as the exponents of p and as g - D1.
             S16Sum s0[2], s1[2], gc[2];
-            const float lw = fast_log2(wk.w);
-            s16_start(s0, tb, wk.pos, wk.run.len, lw - lse.x);
-            s16_start(s1, tb, wk.pos, wk.run.len, lw - lse.y);
+            const float lw = fast_log2(weight);
+            quad_start(s0, cur, tb, lw - lse.x);
+            quad_start(s1, cur, tb, lw - lse.y);
             gc[0].hi = gc[1].hi = f4v{-D1, -D1, -D1, -D1};
             gc[0].lo = gc[1].lo = f4v{0.f, 0.f, 0.f, 0.f};
             qo.scores(s0[0], s1[0], k0, c, qd);
@@ -398,16 +433,12 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
             s16_split_blocks(d1, ds[1]);
             acc.add(k0, k1, c, qd, d0, d1, d);
         }
-        if (wk.more) {
-            __syncthreads();
-            rb = wk.fresh ? 0 : s16_block(rb, 2);
-            if (wk.fresh)
-                bd.template commit<FRESH>(Ks, Vs, tid, 0);
-            else
-                bd.template commit<HK>(Ks, Vs, tid, 16 * s16_block(rb, 3));
-        }
+        bd.commit(other, tid);
+        weight = bd.w;
         __syncthreads();
-        wk.advance();
+        char *t = buf;
+        buf = other, other = t;
+        cur = wk.step();
     }
 
     // (stored after the walk, see dq_d16_kernel)
@@ -434,7 +465,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
                 s16_store4(dq + 16 * cb, x * (one ? 1.f : -lam));
             }
     }
-    if (active) {
+    if (QUAD * u.g + wv < a.Ho) {
         part = point_lanes_sum(part);
         if (lane == 0) a.lam_part[(size_t)bh * a.lam_n + (size_t)ho * ((a.Wo + HQ - 1) / HQ) + w0 / HQ] = part;
     }
@@ -442,28 +473,27 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 }
 
 // ---- backward, dk/dv pass: transposed gather (see dkdv_s16_kernel) ---------------------------------------------------------------------
-template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void dkdv_dsplit_kernel(const DArgs a)
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <= 32 ? 3 : 1) void dkdv_dsplit_kernel(const DArgs a)
 {
-    typedef SplitBand<T, D, PAD> Band_;
+    typedef SplitStage<T, D, PAD> Band_;
     constexpr int S = Band_::S, PITCH = Band_::PITCH, NCB = D / 16;
     extern __shared__ __attribute__((aligned(16))) char h16_lds[];
-    char *Qs = h16_lds, *Gs = h16_lds + Band_::BYTES;
-    float *Ts = reinterpret_cast<float *>(h16_lds + 2 * Band_::BYTES); // [4][FRESH]: log2 w - lse of the two maps, -D1, D1 - D2 of the staged queries
     if ((int)blockIdx.x < a.lam_blocks) {
         diff_sum_lam(a, blockIdx.x, threadIdx.x, 64 * NW, reinterpret_cast<double *>(h16_lds));
         return;
     }
     const int block = blockIdx.x - a.lam_blocks;
 
-    S2_H16_IDS_OF(threadIdx.x, block, a.Wi, a.Hi)
-    const int wv = __builtin_amdgcn_readfirstlane(wave);
-    const int hi = a.sorder[rowsel];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, qd = lane >> 4, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const QuadUnit u = quad_unit(a, block);
+    const int bh = u.bh, b = u.b, h = u.h, w0 = u.w0;
+    const int hi = min(QUAD * u.g + wv, a.Hi - 1);
     const int nk = PAD ? a.dk_ : D, nv = PAD ? a.dv_ : D, d = nk / 2;
     const T *qy = static_cast<const T *>(a.q) + (size_t)b * a.Ho * a.Wo * a.ldq + h * nk;
     const T *gy = static_cast<const T *>(a.dy) + (size_t)b * a.Ho * a.Wo * a.ldg + h * nv;
     const float4 *stats = a.dstats + (size_t)bh * a.Ho * a.Wo;
-    const bool mine = c < nvalid;
-    const size_t pt = (size_t)key_point(a, b, hi, hi / a.kps) + (size_t)(w0 + (mine ? c : 0)) * a.kps;
+    const bool mine = QUAD * u.g + wv < a.Hi && w0 + c < a.Wi;
+    const size_t pt = (size_t)key_point(a, b, hi, a.kps == 1 ? hi : hi / a.kps) + (size_t)(w0 + (mine ? c : 0)) * a.kps;
     float lam = load_as_f32(a.lam, h, a.lam_dtype);
 
     constexpr bool QSCALED = S == 3;
@@ -471,55 +501,37 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     S16Own<T, D, false> vo;
     ko.load(static_cast<const T *>(a.k) + pt * a.ldk + h * nk, nk, qd);
     vo.template load<PAD>(static_cast<const T *>(a.v) + pt * a.ldv + h * nv, nv, qd);
-    typedef typename std::conditional<(D >= 32), f4v, S16Sum>::type Sum;
-    SplitMapSum<Sum, D, S, PAD> dkt;
+    SplitMapSum<f4v, D, S, PAD> dkt;
     dkt.zero();
-    Sum dvt[NCB];
+    f4v dvt[NCB];
     s16_zero(dvt);
-    const float lw = fast_log2(a.quad_w[hi / a.kps]);
+    const float lw = fast_log2(a.quad_w[a.kps == 1 ? hi : hi / a.kps]);
 
-    H16Walk wk;
-    wk.ri = a.soff[hi];
-    wk.rend = a.soff[hi + 1];
-    wk.pos = 0;
-    wk.run = Run{0, 0, 0, 0};
-    wk.w = 1.f;
+    QuadWalk wk;
     Band_ bd;
     float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
     const unsigned lda = a.ldq * a.qps, ldb = a.ldg * a.qps; // elements between two columns of a virtual output latitude
-    auto fetch = [&](const Run &rn, bool fresh) {
-        int c0 = 0;
-        if (fresh) { // longitude of band row 0, in [0, 2 W)
-            c0 = wg0 - rn.ws - rn.len + 1 + a.Wo;
-            while (c0 < 0) c0 += a.Wo;
-        }
-        const int cs = wk.stage(fresh, c0, a.Wo);
-        const size_t row = (size_t)query_row(a, rn.lat, rn.pad);
-        if (fresh)
-            bd.template fetch<FRESH>(qy + row * a.ldq, gy + row * a.ldg, tid, cs, a.Wo, lda, ldb, nk, nv);
-        else
-            bd.template fetch<HK>(qy + row * a.ldq, gy + row * a.ldg, tid, cs, a.Wo, lda, ldb, nk, nv);
-        if (tid < (fresh ? FRESH : HK)) { // the first threads fetch the statistics of the staged rows
-            int col = cs + tid;
-            while (col >= a.Wo) col -= a.Wo;
-            st = stats[(size_t)rn.lat * a.Wo + col];
+    auto fetch = [&]() {
+        const size_t row = quad_row(wk.lat, wk.aux, a.qps, a.Wo);
+        const int cs = wk.column(w0, a.Wo), n = wk.rows();
+        bd.fetch(qy + row * a.ldq, gy + row * a.ldg, tid, cs, a.Wo, n, lda, ldb, nk, nv);
+        int col = cs + min(tid & (HK - 1), n - 1); // (the first threads' are used)
+        if (col >= a.Wo) col -= a.Wo;
+        st = stats[(size_t)wk.lat * a.Wo + col];
+    };
+    auto commit = [&](char *to) {
+        bd.template commit<QSCALED>(to, tid);
+        if (tid < HK) { // -lse of the two maps, -D1, D1 - D2
+            float *t = reinterpret_cast<float *>(to + Band_::BYTES) + tid;
+            t[0] = -st.x, t[HK] = -st.y, t[2 * HK] = -st.z, t[3 * HK] = st.z - st.w;
         }
     };
-    auto commit = [&](bool fresh, int x0) {
-        if (fresh)
-            bd.template commit<FRESH, QSCALED>(Qs, Gs, tid, 0);
-        else
-            bd.template commit<HK, QSCALED>(Qs, Gs, tid, x0);
-        if (tid < (fresh ? FRESH : HK)) {
-            int r = x0 + tid;
-            r -= r >= FRESH ? FRESH : 0;
-            Ts[r] = lw - st.x, Ts[FRESH + r] = lw - st.y, Ts[2 * FRESH + r] = -st.z, Ts[3 * FRESH + r] = st.z - st.w;
-        }
-    };
-    if (wk.ri < wk.rend) {
-        wk.run = a.sruns[wk.ri];
-        fetch(wk.run, true);
-        commit(true, 0);
+    char *buf = h16_lds, *other = h16_lds + Band_::BYTES + HK * 16;
+    wk.start(a, u, wv, lane);
+    QuadStep cur = wk.step();
+    if (cur.some) {
+        fetch();
+        commit(buf);
     }
     __syncthreads();
     ko.settle_();
@@ -527,32 +539,29 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     settle(lam);
 
     const int tb = 4 * qd - c;
-    int rb = 0;
-    while (wk.ri < wk.rend) {
-        wk.plan(a.sruns);
-        if (wk.more) fetch(wk.nrun, wk.fresh);
-        if (active) {
-            const int len = wk.run.len, pos = wk.pos;
-            const int blk[2] = {s16_block(rb, wv), s16_block(s16_block(rb, wv), 1)};
-            const char *q0 = Qs + blk[0] * 16 * PITCH, *q1 = Qs + blk[1] * 16 * PITCH, *g0 = Gs + blk[0] * 16 * PITCH, *g1 = Gs + blk[1] * 16 * PITCH;
+    while (cur.some) {
+        wk.follow();
+        fetch();
+        if (cur.seen()) {
+            const char *q0 = buf, *q1 = buf + 16 * PITCH, *g0 = buf + HK * PITCH, *g1 = buf + (HK + 16) * PITCH;
             // The sums start at the staged statistics, so they end as the exponents of p and as g - D1.
             S16Sum s0[2], s1[2], gc[2];
             f4v step[2];
 #pragma unroll
             for (int qb = 0; qb < 2; qb++) {
-                const float *t = Ts + 16 * blk[qb] + 4 * qd;
-                s0[qb].hi = *reinterpret_cast<const f4v *>(t);
-                s1[qb].hi = *reinterpret_cast<const f4v *>(t + FRESH);
-                gc[qb].hi = *reinterpret_cast<const f4v *>(t + 2 * FRESH);
-                step[qb] = *reinterpret_cast<const f4v *>(t + 3 * FRESH);
+                const float *t = reinterpret_cast<const float *>(buf + Band_::BYTES) + 16 * qb + 4 * qd;
+                s0[qb].hi = *reinterpret_cast<const f4v *>(t) + lw;
+                s1[qb].hi = *reinterpret_cast<const f4v *>(t + HK) + lw;
+                gc[qb].hi = *reinterpret_cast<const f4v *>(t + 2 * HK);
+                step[qb] = *reinterpret_cast<const f4v *>(t + 3 * HK);
                 s0[qb].lo = s1[qb].lo = gc[qb].lo = f4v{0.f, 0.f, 0.f, 0.f};
             }
-            if (pos == 0 || pos + HK > len) { // (rows outside the neighborhood: a probability of zero)
+            if (!cur.inner()) { // (rows outside the neighborhood: a probability of zero)
 #pragma unroll
                 for (int qb = 0; qb < 2; qb++)
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
-                        const bool in = (unsigned)(tb + pos + 16 * qb + v) < (unsigned)len;
+                        const bool in = (unsigned)(tb + cur.pos - cur.d + 16 * qb + v) < (unsigned)cur.l;
                         s0[qb].hi[v] = in ? s0[qb].hi[v] : -INFINITY;
                         s1[qb].hi[v] = in ? s1[qb].hi[v] : -INFINITY;
                     }
@@ -579,13 +588,11 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
             s16_split_blocks(d1, ds[1]);
             dkt.add(q0, q1, c, qd, ps, d1, d);
         }
-        if (wk.more) {
-            __syncthreads();
-            rb = wk.fresh ? 0 : s16_block(rb, 2);
-            commit(wk.fresh, wk.fresh ? 0 : 16 * s16_block(rb, 3));
-        }
+        commit(other);
         __syncthreads();
-        wk.advance();
+        char *t = buf;
+        buf = other, other = t;
+        cur = wk.step();
     }
 
     float check = dkt.check();

@@ -2285,6 +2285,7 @@ template <typename T> __global__ __launch_bounds__(64) void dkdv_mfma_kernel(con
 #include "s2attn_s16.hpp"
 #include "s2attn_s16_ring.hpp"
 #include "s2attn_diff.hpp"
+#include "s2attn_quads.hpp"
 #include "s2attn_diff16.hpp"
 #include "s2attn_diffsplit.hpp"
 
@@ -2593,10 +2594,10 @@ template int launch_diff_points<float>(Which, const DArgs &, hipStream_t);
 template int launch_diff_points<bf16_t>(Which, const DArgs &, hipStream_t);
 template int launch_diff_points<f16_t>(Which, const DArgs &, hipStream_t);
 #endif
-// differential attention, tiles of 64 columns
+// differential attention, tiles of four latitudes by sixteen columns
 template <typename K> int launch_diff_tiles(K kern, Which which, const DArgs &a, int lds, hipStream_t stream)
 {
-    const long tiles = (which == DKDV ? (a.dk ? (long)a.Hi * ((a.Wi + WQ - 1) / WQ) : 0) : (long)a.Ho * ((a.Wo + WQ - 1) / WQ)) * a.B * a.nh;
+    const long tiles = which == DKDV && !a.dk ? 0 : (long)a.q_groups * ((a.Wi + HQ - 1) / HQ) * a.B * a.nh;
     const long nblocks = tiles + (which == DKDV ? a.lam_blocks : 0);
     if (nblocks >= (1L << 32) / (64 * NW)) return s2attn_fail(S2ATTN_E_UNSUPPORTED, "problem needs %ld workgroups, more than one grid holds", nblocks);
     if (nblocks == 0) return S2ATTN_OK;
@@ -2613,7 +2614,7 @@ template <typename K> int launch_diff_tiles(K kern, Which which, const DArgs &a,
 template <typename T, int D, bool PAD> int launch_d16(Which which, const DArgs &a, hipStream_t stream)
 {
     void (*const kern)(const DArgs) = which == FWD ? fwd_d16_kernel<T, D, PAD> : which == DQ ? dq_d16_kernel<T, D, PAD> : dkdv_d16_kernel<T, D, PAD>;
-    return launch_diff_tiles(kern, which, a, d16_lds_bytes<D>(), stream);
+    return launch_diff_tiles(kern, which, a, d16_lds_bytes<D>(which == DKDV), stream);
 }
 #endif
 #if S2_PART == 8
@@ -3466,6 +3467,11 @@ int diff_args(DArgs &a, const void *k, const void *v, const void *q, const void 
     rc = check_plan(plan, &sh);
     if (rc != S2ATTN_OK) return rc;
     fill_args(a, plan, &sh, quad_weights);
+    if (const int at = plan->header[S2ATTN_PH_QUADS]) { // (0: a plan without them)
+        if (at < S2ATTN_PLAN_HEADER_INTS || (int64_t)at + s2_quad_layout(a.Ho, a.Hi).bands + 8 > plan->header[S2ATTN_PH_TOTAL])
+            return s2attn_fail(S2ATTN_E_INVALID, "plan header: the bands of the differential kernels at %d lie outside the plan", at);
+        a.quads = plan->data + at;
+    }
     a.k = k, a.v = v, a.q = q, a.lam = lam, a.lam_dtype = lam_dtype;
     return S2ATTN_OK;
 }
@@ -3473,7 +3479,7 @@ int diff_args(DArgs &a, const void *k, const void *v, const void *q, const void 
 template <typename T> int diff_family_t(const DArgs &a, size_t alignment)
 {
     const int c = std::max(a.dk_, a.dv_);
-    if (a.Wi < HK) return S2ATTN_FAMILY_VECTOR;
+    if (a.Wi < HK || !a.quads) return S2ATTN_FAMILY_VECTOR;
     if constexpr (!std::is_same<T, float>::value) {
         const bool strides = (a.ldk | a.ldv | a.ldq | a.ldy | a.ldg | a.lddk | a.lddv | a.lddq) % 8 == 0;
         if (a.dk_ % 16 == 0 && a.dv_ % 8 == 0 && c <= 128 && strides && alignment % 16 == 0) return S2ATTN_FAMILY_16BIT;
@@ -3493,10 +3499,28 @@ size_t common_alignment(std::initializer_list<const void *> ptrs)
     for (const void *p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
     return bits ? bits & (~bits + 1) : 4096;
 }
+QuadDiv quad_divisor(long d)
+{
+    QuadDiv q = {0, 0};
+    if (d >= 1L << 24) return q; // (such a launch is refused)
+    for (q.s = 24; 1L << (q.s - 24) < d;) q.s++;
+    q.m = (unsigned)((1UL << q.s) / (unsigned long)d) + 1;
+    return q;
+}
 template <typename T> int launch_diff_t(Which which, int family, DArgs &a, hipStream_t stream)
 {
     a.lam_n = a.Ho * (family == S2ATTN_FAMILY_VECTOR ? a.Wo : (a.Wo + HQ - 1) / HQ);
     a.lam_blocks = which == DKDV && a.dlam ? a.nh : 0;
+    if (a.quads) {
+        const s2_quad_layout at(a.Ho, a.Hi);
+        a.q_groups = ((which == DKDV ? a.Hi : a.Ho) + QUAD - 1) / QUAD;
+        a.q_list = a.quads + (which == DKDV ? at.scatter : 0);
+        a.q_bands = a.quads + at.bands;
+        const int bh = a.B * a.nh, nt = (a.Wi + HQ - 1) / HQ;
+        a.q_first = quad_divisor(bh % 8 == 0 ? (long)a.q_groups * nt : bh);
+        a.q_tiles = quad_divisor(nt);
+        a.q_head = quad_divisor(a.nh);
+    }
     if constexpr (!std::is_same<T, float>::value) {
         if (family == S2ATTN_FAMILY_16BIT) {
             const int c = std::max(a.dk_, a.dv_);

@@ -249,6 +249,73 @@ bool merge_pair(const Group &A, const Group &B, int W, bool scatter, std::vector
     return true;
 }
 
+// ---- bands that four latitudes share ---------------------------------------------------------------------------------------------
+// The differential kernels work on four adjacent (virtual) latitudes at a time, each in a wavefront of its own, and stage what any of them sees.
+// Per group of four latitudes and per latitude of the other grid their runs are joined to one band, eight ints:
+//   lat, aux   the other latitude, virtual and real (as in the runs)
+//   ws, len    its columns ws + t + w for tile column w, t in [0, len)
+//   dl[4]      per latitude of the group d << 16 | l: it sees t in [d, d + l)
+// Runs that lie too far apart to gain by it, or several of one pair of latitudes, are bands of their own.  A group is four ints: its number, its
+// bands first .. last, 0.
+struct QuadBand {
+    int32_t v[8];
+};
+struct QuadGroup {
+    int32_t number, first, last, zero;
+};
+constexpr int QUAD = 4;
+
+// start: first column of a run as a band of the grouping has it.  Groups by decreasing number of steps, in classes inside which neighbors stay next to
+// each other (see order_rows).
+template <typename Start>
+void build_quads(const std::vector<int32_t> &off, const std::vector<int32_t> &runs, int nv, int W, Start start, std::vector<QuadGroup> *groups, std::vector<QuadBand> *out)
+{
+    std::vector<int32_t> steps;
+    const size_t first_group = groups->size();
+    struct Member {
+        int32_t lat, layer, i, s, len, aux;
+    };
+    std::vector<Member> ms;
+    for (int first = 0; first < nv; first += QUAD) {
+        ms.clear();
+        for (int i = 0; i < std::min(QUAD, nv - first); i++) {
+            const size_t begin = ms.size();
+            for (int32_t r = off[first + i]; r < off[first + i + 1]; r++)
+                ms.push_back({runs[4 * (size_t)r], 0, i, start(r), runs[4 * (size_t)r + 2], runs[4 * (size_t)r + 3]});
+            std::stable_sort(ms.begin() + begin, ms.end(), [](const Member &x, const Member &y) { return x.lat < y.lat; });
+            for (size_t m = begin + 1; m < ms.size(); m++)
+                if (ms[m].lat == ms[m - 1].lat) ms[m].layer = ms[m - 1].layer + 1;
+        }
+        std::stable_sort(ms.begin(), ms.end(), [](const Member &x, const Member &y) { return x.lat != y.lat ? x.lat < y.lat : x.layer < y.layer; });
+        const int32_t first_band = (int32_t)out->size();
+        int32_t work = 0;
+        size_t m = 0;
+        while (m < ms.size()) {
+            int32_t d[QUAD] = {0, 0, 0, 0}, len[QUAD] = {0, 0, 0, 0}, lo = ms[m].s, hi = lo + ms[m].len;
+            const Member &head = ms[m];
+            for (; m < ms.size() && ms[m].lat == head.lat && len[ms[m].i] == 0; m++) {
+                int32_t at = ms[m].s;
+                const int32_t want = lo + hi - ms[m].len; // (twice the start that centers it on the band so far)
+                while (2 * at - want > W) at -= W;
+                while (want - 2 * at > W) at += W;
+                const int32_t nlo = std::min(lo, at), nhi = std::max(hi, at + ms[m].len), longest = std::max(hi - lo, ms[m].len);
+                if (nhi - nlo > longest + 16 && nhi - nlo > 2 * longest) break;
+                lo = nlo, hi = nhi;
+                d[ms[m].i] = at, len[ms[m].i] = ms[m].len;
+            }
+            QuadBand q = {{head.lat, head.aux, ((lo % W) + W) % W, hi - lo, 0, 0, 0, 0}};
+            for (int i = 0; i < QUAD; i++)
+                if (len[i]) q.v[4 + i] = (d[i] - lo) << 16 | len[i];
+            out->push_back(q);
+            work += (hi - lo + 15 + 31) / 32;
+        }
+        groups->push_back({first / QUAD, first_band, (int32_t)out->size(), 0});
+        steps.push_back(work);
+    }
+    std::stable_sort(groups->begin() + first_group, groups->end(),
+                     [&](const QuadGroup &a, const QuadGroup &b) { return cost_class(steps[(size_t)a.number]) > cost_class(steps[(size_t)b.number]); });
+}
+
 // Work list of one grouping for the hybrid kernels: items (latitude, pair index or -1), long-run latitudes and short-run
 // units (single latitudes or pairs) merged by share of work as in order_rows.
 void build_items(const int32_t *off, const int32_t *runs, int ngroups, int W, bool scatter, const std::vector<RowCost> &cost,
@@ -380,6 +447,15 @@ int build_blob(const int64_t *col_idx, const int64_t *row_off, int64_t nnz, int 
     h[S2ATTN_PH_SCATTER_PAIR_RUNS] = append(blob, spruns.data(), spruns.size());
     h[S2ATTN_PH_SCATTER_NPAIRS] = (int32_t)spoff.size() - 1;
     h[S2ATTN_PH_GATHER_SPAN] = append(blob, gspan.data(), gspan.size());
+    if (W < 0x3f00) { // (a band's numbers are packed in pairs)
+        std::vector<QuadGroup> groups;
+        std::vector<QuadBand> bands;
+        build_quads(goff, gruns, nvout, W, [&](int32_t r) { return gruns[4 * (size_t)r + 1]; }, &groups, &bands);
+        build_quads(soff, sruns, nvin, W, [&](int32_t r) { return ((1 - sruns[4 * (size_t)r + 1] - sruns[4 * (size_t)r + 2]) % W + W) % W; }, &groups, &bands);
+        bands.push_back({{0, 0, 0, 0, 0, 0, 0, 0}}); // (kernels read one band ahead)
+        h[S2ATTN_PH_QUADS] = append(blob, &groups[0].number, 4 * groups.size()); // the parts start where s2_quad_layout says
+        append(blob, bands[0].v, 8 * bands.size());
+    }
     while (blob.size() % 4) blob.push_back(0);
     if (blob.size() > 0x7fffffffULL) return s2attn_fail(S2ATTN_E_UNSUPPORTED, "the plan needs %zu ints, more than its 32-bit offsets index", blob.size());
     h[S2ATTN_PH_TOTAL] = (int32_t)blob.size();
