@@ -5,8 +5,8 @@
 //
 // The row of k (q) holds both maps' channels and is staged once; map i's scores take the 32-channel blocks it has channels in, with the other map's
 // channels zero on the side that stays in registers.  <dy, v>, the masks, the staged rows and the transposed reads of v serve both maps.
-// Sums of probabilities (forward) and of dS and of P (dq pass: the corrections of D, see diff_point_dq) are further products with the
-// staged rows or with ones, so they are of the rounded values that the other products take.
+// Sums of probabilities (forward) and of dS and of P (dq pass: the corrections of D, see diff_point_dq) are of the rounded values that
+// the products take: pairwise products with one (d16_sum: products on the matrix cores hold ten more registers), or with the staged rows.
 //
 // Shape domain: ck a multiple of 8, cv a multiple of 8, 2 ck and cv at most D (a tile is D channels wide, 32, 64 or 128; zeros are staged past
 // a head's channels and never stored; PAD = false: 2 ck = cv = D), at least 32 columns per virtual latitude, rows 16-byte aligned.
@@ -111,10 +111,20 @@ template <typename M> __device__ inline uint4 d16_pack(const f4v (&x)[2])
 {
     return make_uint4(M::pack2(x[0][0], x[0][1]), M::pack2(x[0][2], x[0][3]), M::pack2(x[1][0], x[1][1]), M::pack2(x[1][2], x[1][3]));
 }
-template <typename M> __device__ inline uint4 d16_ones()
+// s + the sum of eight values as they were rounded
+template <typename T> __device__ inline float d16_sum(float s, uint4 p)
 {
-    const unsigned one = M::pack2(1.f, 1.f);
-    return make_uint4(one, one, one, one);
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const unsigned w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (std::is_same<T, bf16_t>::value)
+            s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w[i]), b2{(__bf16)1.f, (__bf16)1.f}, s, false);
+        else
+            s = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w[i]), h2{(_Float16)1.f, (_Float16)1.f}, s, false);
+    }
+    return s;
 }
 
 // The kernel's arguments again and the lanes counted anew, as point_args() has it
@@ -144,11 +154,12 @@ template <typename T, int D, Which PASS> __device__ __forceinline__ void diff_re
     }
 }
 
-// Registers decide how many wavefronts a SIMD holds; where the compiler comes close to one more by itself, the launch bounds ask for it (dk/dv pass, 64
-// channels, 361x720: 143 registers and three 379 us, 128 and four 326).
+// Registers decide how many wavefronts a SIMD holds; where the compiler comes close to one more by itself, the launch bounds ask for it.  361x720, 64
+// channels: dk/dv pass 143 registers, three wavefronts 379 us / 128, four 326; dq 356 / 330 (four); forward 110, four 287 / 96, five 267.  (Asked for more
+// than fits, the loop spills: the forward with fourteen registers too few took 441.)
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
-template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) void fwd_d16_kernel(const DArgs a)
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D == 32 ? 6 : D == 128 ? 3 : PAD ? 4 : 5) void fwd_d16_kernel(const DArgs a)
 {
     typedef DiffStage<D, PAD> Tile;
     typedef H16<T> M;
@@ -166,15 +177,13 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 
     DiffOwn<M, D, PAD> own;
     own.load(static_cast<const char *>(a.q) + (pt * a.ldq + (size_t)h * nk) * 2, qd, d);
-    f4v acc[2][NCB], Z[2]; // Y^T of each map: register v of block cb is channel 16 cb + 4 qd + v of column c; sums of probabilities
+    f4v acc[2][NCB]; // Y^T of each map: register v of block cb is channel 16 cb + 4 qd + v of column c; sums of probabilities
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        Z[i] = f4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int cb = 0; cb < NCB; cb++) acc[i][cb] = f4v{0.f, 0.f, 0.f, 0.f};
     }
-    float m[2] = {NEG_BIG, NEG_BIG};
-    const uint4 ones = d16_ones<M>();
+    float m[2] = {NEG_BIG, NEG_BIG}, Z[2] = {0.f, 0.f};
 
     QuadWalk wk;
     Tile bd = {}; // the next step's rows, on their way
@@ -245,7 +254,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 #pragma unroll
                     for (int v = 0; v < 4; v++) sc[i][kb][v] = fast_exp2(fmaf(sc[i][kb][v], LOG2E, sh)); // masked: exp2(-inf) = 0
                 p[i] = d16_pack<M>(sc[i]);
-                Z[i] = M::mfma(ones, p[i], Z[i]);
+                Z[i] = d16_sum<T>(Z[i], p[i]); // this lane's share
             }
 #pragma unroll
             for (int cb = 0; cb < NCB; cb++) {
@@ -262,12 +271,12 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
         cur = wk.step();
     }
 
-    float check = Z[0][0] + Z[1][0];
+    const float z0 = h16_quarter_sum(Z[0]), z1 = h16_quarter_sum(Z[1]);
+    float check = z0 + z1;
 #pragma unroll
     for (int cb = 0; cb < NCB; cb++) check += point_sum(acc[0][cb] + acc[1][cb]);
     const unsigned redo = point_columns(mine && not_finite(check));
     if (mine) {
-        const float z0 = Z[0][0], z1 = Z[1][0];
         if (a.lse2 && qd == 0)
             a.lse2[((size_t)bh * a.Ho + ho) * a.Wo + w0 + c] = make_float2(z0 == 0.f ? INFINITY : m[0] + fast_log2(z0), z1 == 0.f ? INFINITY : m[1] + fast_log2(z1));
         const float i0 = z0 == 0.f ? 0.f : 1.0f / z0, i1 = z1 == 0.f ? 0.f : 1.0f / z1, lam = load_as_f32(a.lam, h, a.lam_dtype);
@@ -286,7 +295,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
 
 // ---- backward, dq pass -----------------------------------------------------------------------------------------------------------
 // Per step and map S^T = K Q^T; G^T = V dY^T once; dQ^T += K^T dS^T, and AK^T += K^T P^T and sum dS for the corrections of D.
-template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <= 64 && !PAD ? 4 : 1) void dq_d16_kernel(const DArgs a)
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D == 64 && !PAD ? 4 : 1) void dq_d16_kernel(const DArgs a)
 {
     typedef DiffStage<D, PAD> Tile;
     typedef H16<T> M;
@@ -329,8 +338,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
 
     DiffSum<M, D, PAD> acc, ak;
     acc.zero(), ak.zero();
-    f4v off[2] = {f4v{0.f, 0.f, 0.f, 0.f}, f4v{0.f, 0.f, 0.f, 0.f}};
-    const uint4 ones = d16_ones<M>();
+    float off[2] = {0.f, 0.f};
 
     QuadWalk wk;
     Tile bd = {}; // the next step's rows, on their way
@@ -386,8 +394,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
                     ds[1][kb][v] = sc[1][kb][v] * (gc[kb][v] + step21);
                 }
             const uint4 p0 = d16_pack<M>(sc[0]), p1 = d16_pack<M>(sc[1]), d0 = d16_pack<M>(ds[0]), d1 = d16_pack<M>(ds[1]);
-            off[0] = M::mfma(ones, d0, off[0]);
-            off[1] = M::mfma(ones, d1, off[1]);
+            off[0] = d16_sum<T>(off[0], d0), off[1] = d16_sum<T>(off[1], d1); // this lane's share
 #pragma unroll
             for (int cb = 0; cb < NCB; cb++) {
                 const uint4 kt = h16_read_transposed<PITCH>(kblk[0], kblk[1], cb, c, qd);
@@ -410,7 +417,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
 
     // (stored after the walk: a global store ahead of the loop would turn the loop's scalar loads of runs and weights,
     // which the compiler only uses while nothing in the kernel can have written memory, into vector loads with waits)
-    const float o0 = off[0][0], o1 = off[1][0];
+    const float o0 = h16_quarter_sum(off[0]), o1 = h16_quarter_sum(off[1]);
     float check = o0 + o1;
 #pragma unroll
     for (int cb = 0; cb < NCB; cb++) check += point_sum(acc.acc[cb] + ak.acc[cb]);
@@ -443,7 +450,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
 // Per step and map S = Q K^T; G = dY V^T once; dV^T += dY^T (P1 - lam P2) once; dK^T += Q^T dS.
 // The statistics of the staged queries lie behind the buffers, log2 w - lse of the two maps, -D1 and D1 - D2, each for 32 rows, so a lane reads
 // those of its four queries at once.  (The key's log2 w is added to the first two in 32 bits.)
-template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <= 32 ? 5 : D <= 64 ? 4 : 1) void dkdv_d16_kernel(const DArgs a)
+template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, PAD || D == 128 ? 1 : D == 64 ? 4 : 5) void dkdv_d16_kernel(const DArgs a)
 {
     typedef DiffStage<D, PAD> Tile;
     typedef H16<T> M;

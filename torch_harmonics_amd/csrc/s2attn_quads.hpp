@@ -7,7 +7,7 @@
 //
 // Rows staged for 64 points, disk of radius R rings, arcs of a columns: (2 R + 4) (15 + a); with a latitude's 64 columns in the four wavefronts
 // (2 R + 1) (63 + a), in a ring of 128 (80) rows with two barriers a run.  Forward, dq and dk/dv took, us, that way / this way: 361x720 bf16 4 x 64
-// channels, R = 2: 269 / 287, 341 / 343, 369 / 326; 180x360 from 90x180 bf16 2 x 128 channels: 92 / 56, 98 / 67, 142 / 120; 128x256 fp32 4 x 32 channels
+// channels, R = 2: 269 / 267, 341 / 330, 369 / 326; 180x360 from 90x180 bf16 2 x 128 channels: 92 / 56, 98 / 68, 142 / 120; 128x256 fp32 4 x 32 channels
 // R = 4: 250 / 205, 252 / 220, 303 / 279; 91x180 bf16 forward alone, which is as long as its longest walk: 24 / 26.
 //
 // Two buffers, one barrier a step.  Bound by issue: vector instructions keep the SIMDs busy half the time, matrix instructions a tenth (16-bit) to a
