@@ -62,7 +62,7 @@ int s2attn_fail(int code, const char *fmt, ...)
 }
 
 extern "C" const char *s2attn_last_error(void) { return g_err; }
-extern "C" int s2attn_abi_version(void) { return 15; }
+extern "C" int s2attn_abi_version(void) { return 16; }
 #endif
 
 namespace s2 {
