@@ -1,5 +1,7 @@
 """The bands that four latitudes share cover exactly the pairs of the CSR."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -84,3 +86,30 @@ def test_the_order_of_psi_does_not_matter():
     moved = torch.cat([torch.tensor(sorted(c.tolist(), key=lambda x: (x // 40, (x % 40 + 20) % 40)), dtype=torch.int64) for c in col.split((roff[1:] - roff[:-1]).tolist())])
     assert not torch.equal(col, moved)
     assert check(col, roff, (12, 40), (12, 40)) == check(moved, roff, (12, 40), (12, 40))
+
+
+@pytest.mark.parametrize(
+    "dtype,d,cv,nlon,alignment,want",
+    [("fp32", 16, 32, 40, 4, "split"), ("fp32", 16, 32, 31, 4, "vector"), ("fp32", 3, 32, 40, 4, "vector"), ("fp32", 64, 128, 40, 4, "split"), ("fp32", 68, 128, 40, 4, "vector"),
+     ("bf16", 32, 64, 40, 16, "16bit"), ("bf16", 32, 64, 40, 8, "split"), ("bf16", 20, 36, 40, 16, "split"), ("fp16", 64, 128, 40, 16, "16bit"), ("fp16", 64, 128, 40, 8, "vector"), ("bf16", 16, 32, 16200, 16, "vector")],
+)  # fmt: skip
+def test_families_of_kernels(dtype, d, cv, nlon, alignment, want):
+    """What a problem's widths, columns and alignment lead to; grids too wide for the bands' packed numbers have none."""
+    lib = _lib.load()
+    col, roff = torch.arange(-2, 3) % nlon, torch.tensor([0, 5, 5])
+    plan = build_host_blob(col, roff, 2, nlon, 2, nlon)
+    assert (plan.header[_lib.PH["QUADS"]] > 0) == (nlon < 0x3F00)
+    shape = _lib.ShapeStruct(batch=1, num_heads=2, nlat_in=2, nlon_in=nlon, nlat_out=2, nlon_out=nlon, ck=d, cv=cv, dtype=["fp32", "bf16", "fp16"].index(dtype))
+    rc = lib.s2attn_diff_family(ctypes.byref(plan.struct), ctypes.byref(shape), alignment)
+    assert _lib.FAMILIES[_lib.check(rc, "family")] == want
+
+
+def test_a_header_that_points_outside_the_plan_is_refused():
+    lib = _lib.load()
+    plan = build_host_blob(torch.arange(5), torch.tensor([0, 5, 5]), 2, 40, 2, 40)
+    shape = _lib.ShapeStruct(batch=1, num_heads=2, nlat_in=2, nlon_in=40, nlat_out=2, nlon_out=40, ck=16, cv=32, dtype=0)
+    bad = _lib.PlanStruct.make(plan.blob.data_ptr(), list(plan.header))
+    for at in (-5, 3, int(plan.header[_lib.PH["TOTAL"]]) - 4):
+        bad.header[_lib.PH["QUADS"]] = at
+        assert lib.s2attn_diff_family(ctypes.byref(bad), ctypes.byref(shape), 16) == -1
+        assert b"bands" in lib.s2attn_last_error()
