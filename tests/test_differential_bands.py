@@ -32,10 +32,16 @@ def pairs_of(groups, bands, nv, W, sigma, rho, shape):
         for band in bands[begin:end].tolist():
             lat, aux, ws, ln = band[:4]
             assert aux == lat // rho and 0 <= ws < W
-            first, last = [], []
+            first, last, rings = [], [], False
             for i in range(4):
                 vo, d, n = 4 * g + i, band[4 + i] >> 16, band[4 + i] & 0xFFFF
                 if n == 0:
+                    continue
+                if n == 0xFFFF:  # the whole ring: positions 0 .. W, seen by all columns of a tile wherever it is
+                    assert vo < nv and d == 0 and ln + 15 >= W
+                    rings = True
+                    own, other = np.meshgrid((vo // sigma) * sigma * W + vo % sigma + w * sigma, (lat // rho) * rho * W + lat % rho + w * rho)
+                    np.add.at(M, (own, other), 1)
                     continue
                 assert vo < nv and 0 <= d and d + n <= ln
                 first.append(d), last.append(d + n)
@@ -43,7 +49,10 @@ def pairs_of(groups, bands, nv, W, sigma, rho, shape):
                     own = (vo // sigma) * sigma * W + vo % sigma + w * sigma
                     other = (lat // rho) * rho * W + lat % rho + (ws + t + w) % W * rho
                     np.add.at(M, (own, other), 1)
-            assert min(first) == 0 and max(last) == ln
+            if first:
+                assert min(first) == 0 and (max(last) == ln or rings and ln == max(max(last), W - 15))
+            else:
+                assert rings and ln == max(1, W - 15)
     return M
 
 

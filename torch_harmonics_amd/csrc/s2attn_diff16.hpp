@@ -191,7 +191,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D =
     auto fetch = [&]() {
         const size_t row = quad_row(wk.lat, wk.aux, a.kps, a.Wi);
         bd.w = a.quad_w[wk.aux + wk.zero];
-        bd.fetch(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, wk.column(w0, a.Wi), a.Wi, wk.rows(), lda, ldb, nk, nv);
+        bd.fetch(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, wk.column(w0), a.Wi, wk.rows(), lda, ldb, nk, nv);
     };
     char *buf = h16_lds, *other = h16_lds + Tile::BYTES;
     wk.start(a, u, wv, lane);
@@ -217,7 +217,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D =
                 sc[0][kb] = sc[1][kb] = f4v{0.f, 0.f, 0.f, 0.f};
                 own.scores(sc[0][kb], sc[1][kb], kblk[kb], c, qd);
             }
-            const int tb = cur.pos - cur.d + 4 * qd - c; // neighbor index of element (kb, v): tb + 16 kb + v
+            const int tb = cur.first(c) + 4 * qd; // neighbor index of element (kb, v): tb + 16 kb + v
             if (!cur.inner()) {
 #pragma unroll
                 for (int kb = 0; kb < 2; kb++)
@@ -346,7 +346,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D =
     auto fetch = [&]() {
         const size_t row = quad_row(wk.lat, wk.aux, a.kps, a.Wi);
         bd.w = a.quad_w[wk.aux + wk.zero];
-        bd.fetch(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, wk.column(w0, a.Wi), a.Wi, wk.rows(), lda, ldb, nk, nv);
+        bd.fetch(kx + 2 * row * a.ldk, vx + 2 * row * a.ldv, tid, wk.column(w0), a.Wi, wk.rows(), lda, ldb, nk, nv);
     };
     char *buf = h16_lds, *other = h16_lds + Tile::BYTES;
     wk.start(a, u, wv, lane);
@@ -380,7 +380,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D =
 #pragma unroll
                 for (int s = 0; s < NS; s++) gc[kb] = M::mfma(h16_read_row<PITCH>(vblk[kb], s, c, qd), gop[s], gc[kb]);
             }
-            const int tb = cur.pos - cur.d + 4 * qd - c;
+            const int tb = cur.first(c) + 4 * qd;
             const bool inner = cur.inner(); // every element of the step is a neighbor: no band mask
             f4v ds[2][2];
 #pragma unroll
@@ -491,7 +491,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, PAD
     const unsigned lda = 2u * a.ldq * a.qps, ldb = 2u * a.ldg * a.qps; // bytes between two columns of a virtual output latitude
     auto fetch = [&]() {
         const size_t row = quad_row(wk.lat, wk.aux, a.qps, a.Wo);
-        const int cs = wk.column(w0, a.Wo), n = wk.rows();
+        const int cs = wk.column(w0), n = wk.rows();
         bd.fetch(qy + 2 * row * a.ldq, gy + 2 * row * a.ldg, tid, cs, a.Wo, n, lda, ldb, nk, nv);
         int col = cs + min(tid & (HK - 1), n - 1); // (the first threads' are used)
         if (col >= a.Wo) col -= a.Wo;
@@ -534,7 +534,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, PAD
 #pragma unroll
                 for (int s = 0; s < NS; s++) gc[qb] = M::mfma(h16_read_row<PITCH>(gblk[qb], s, c, qd), vop[s], gc[qb]);
             }
-            const int tb = cur.pos - cur.d + 4 * qd - c; // r - c of element (qb, v): tb + 16 qb + v
+            const int tb = cur.first(c) + 4 * qd; // r - c of element (qb, v): tb + 16 qb + v
             const bool inner = cur.inner(); // every element of the step is a (query, key) pair of the band
             f4v ds[2][2], co[2];
 #pragma unroll

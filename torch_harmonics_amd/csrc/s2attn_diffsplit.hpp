@@ -206,12 +206,12 @@ template <typename T, int D, bool PAD> struct SplitStage {
 template <typename T, int D> constexpr int dsplit_lds_bytes(bool stats) { return 2 * (SplitStage<T, D, false>::BYTES + (stats ? HK * 16 : 0)); }
 
 // Start values of a step's scores: `start` where the point sees the position
-__device__ inline void quad_start(S16Sum (&sc)[2], const QuadStep &cur, int tb, float start)
+__device__ inline void quad_start(S16Sum (&sc)[2], const QuadStep &cur, int c, int qd, float start)
 {
     sc[0].lo = sc[1].lo = f4v{0.f, 0.f, 0.f, 0.f};
     sc[0].hi = sc[1].hi = f4v{start, start, start, start};
     if (!cur.inner()) {
-        tb += cur.pos - cur.d;
+        const int tb = cur.first(c) + 4 * qd;
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -249,7 +249,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
     auto fetch = [&]() {
         const size_t row = quad_row(wk.lat, wk.aux, a.kps, a.Wi);
         bd.w = a.quad_w[wk.aux + wk.zero];
-        bd.fetch(kx + row * a.ldk, vx + row * a.ldv, tid, wk.column(w0, a.Wi), a.Wi, wk.rows(), lda, ldb, nk, nv);
+        bd.fetch(kx + row * a.ldk, vx + row * a.ldv, tid, wk.column(w0), a.Wi, wk.rows(), lda, ldb, nk, nv);
     };
     char *buf = h16_lds, *other = h16_lds + Band_::BYTES;
     wk.start(a, u, wv, lane);
@@ -263,7 +263,6 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
     __syncthreads();
     own.settle_();
 
-    const int tb = 4 * qd - c;
     while (cur.some) {
         wk.follow();
         fetch();
@@ -272,8 +271,8 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
             // The sums start at log2 w - m, so they end as the exponents of the probabilities.
             S16Sum s0[2], s1[2];
             const float lw = fast_log2(weight);
-            quad_start(s0, cur, tb, lw - m[0]);
-            quad_start(s1, cur, tb, lw - m[1]);
+            quad_start(s0, cur, c, qd, lw - m[0]);
+            quad_start(s1, cur, c, qd, lw - m[1]);
             own.scores(s0[0], s1[0], k0, c, qd);
             own.scores(s0[1], s1[1], k1, c, qd);
             f4v p[2][2] = {{s16_value(s0[0]), s16_value(s0[1])}, {s16_value(s1[0]), s16_value(s1[1])}};
@@ -404,7 +403,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     auto fetch = [&]() {
         const size_t row = quad_row(wk.lat, wk.aux, a.kps, a.Wi);
         bd.w = a.quad_w[wk.aux + wk.zero];
-        bd.fetch(kx + row * a.ldk, vx + row * a.ldv, tid, wk.column(w0, a.Wi), a.Wi, wk.rows(), lda, ldb, nk, nv);
+        bd.fetch(kx + row * a.ldk, vx + row * a.ldv, tid, wk.column(w0), a.Wi, wk.rows(), lda, ldb, nk, nv);
     };
     char *buf = h16_lds, *other = h16_lds + Band_::BYTES;
     wk.start(a, u, wv, lane);
@@ -421,7 +420,6 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
     settle(lse.x), settle(lse.y);
     const float step21 = D1 - D2; // g - D2 = (g - D1) + (D1 - D2)
 
-    const int tb = 4 * qd - c;
     while (cur.some) {
         wk.follow();
         fetch();
@@ -430,8 +428,8 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW) voi
             // The sums start at log2 w - lse and at -D1, so they end as the exponents of p and as g - D1.
             S16Sum s0[2], s1[2], gc[2];
             const float lw = fast_log2(weight);
-            quad_start(s0, cur, tb, lw - lse.x);
-            quad_start(s1, cur, tb, lw - lse.y);
+            quad_start(s0, cur, c, qd, lw - lse.x);
+            quad_start(s1, cur, c, qd, lw - lse.y);
             gc[0].hi = gc[1].hi = f4v{-D1, -D1, -D1, -D1};
             gc[0].lo = gc[1].lo = f4v{0.f, 0.f, 0.f, 0.f};
             qo.scores(s0[0], s1[0], k0, c, qd);
@@ -541,7 +539,7 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
     const unsigned lda = a.ldq * a.qps, ldb = a.ldg * a.qps; // elements between two columns of a virtual output latitude
     auto fetch = [&]() {
         const size_t row = quad_row(wk.lat, wk.aux, a.qps, a.Wo);
-        const int cs = wk.column(w0, a.Wo), n = wk.rows();
+        const int cs = wk.column(w0), n = wk.rows();
         bd.fetch(qy + row * a.ldq, gy + row * a.ldg, tid, cs, a.Wo, n, lda, ldb, nk, nv);
         int col = cs + min(tid & (HK - 1), n - 1); // (the first threads' are used)
         if (col >= a.Wo) col -= a.Wo;
@@ -566,7 +564,6 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
     vo.settle_();
     settle(lam);
 
-    const int tb = 4 * qd - c;
     while (cur.some) {
         wk.follow();
         fetch();
@@ -584,12 +581,13 @@ template <typename T, int D, bool PAD> __global__ __launch_bounds__(64 * NW, D <
                 step[qb] = *reinterpret_cast<const f4v *>(t + 3 * HK);
                 s0[qb].lo = s1[qb].lo = gc[qb].lo = f4v{0.f, 0.f, 0.f, 0.f};
             }
+            const int tb = cur.first(c) + 4 * qd;
             if (!cur.inner()) { // (rows outside the neighborhood: a probability of zero)
 #pragma unroll
                 for (int qb = 0; qb < 2; qb++)
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
-                        const bool in = (unsigned)(tb + cur.pos - cur.d + 16 * qb + v) < (unsigned)cur.l;
+                        const bool in = (unsigned)(tb + 16 * qb + v) < (unsigned)cur.l;
                         s0[qb].hi[v] = in ? s0[qb].hi[v] : -INFINITY;
                         s1[qb].hi[v] = in ? s1[qb].hi[v] : -INFINITY;
                     }

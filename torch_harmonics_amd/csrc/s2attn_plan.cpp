@@ -254,7 +254,9 @@ bool merge_pair(const Group &A, const Group &B, int W, bool scatter, std::vector
 // Per group of four latitudes and per latitude of the other grid their runs are joined to one band, eight ints:
 //   lat, aux   the other latitude, virtual and real (as in the runs)
 //   ws, len    its columns ws + t + w for tile column w, t in [0, len)
-//   dl[4]      per latitude of the group d << 16 | l: it sees t in [d, d + l)
+//   dl[4]      per latitude of the group d << 16 | l: it sees t in [d, d + l); QUAD_RING: the whole ring, once
+// A band is staged as positions t = 0 .. len + 15 for sixteen columns, column w0 + c of which sees t - c in [d, d + l).  A whole ring has no first
+// column: whichever positions 0 .. W are, all sixteen see them, and W positions do where an arc as long would need W + 15.
 // Runs that lie too far apart to gain by it, or several of one pair of latitudes, are bands of their own.  A group is four ints: its number, its
 // bands first .. last, 0.
 struct QuadBand {
@@ -263,7 +265,7 @@ struct QuadBand {
 struct QuadGroup {
     int32_t number, first, last, zero;
 };
-constexpr int QUAD = 4;
+constexpr int QUAD = 4, QUAD_RING = 0xffff;
 
 // start: first column of a run as a band of the grouping has it.  Groups by decreasing number of steps, in classes inside which neighbors stay next to
 // each other (see order_rows).
@@ -291,10 +293,16 @@ void build_quads(const std::vector<int32_t> &off, const std::vector<int32_t> &ru
         int32_t work = 0;
         size_t m = 0;
         while (m < ms.size()) {
-            int32_t d[QUAD] = {0, 0, 0, 0}, len[QUAD] = {0, 0, 0, 0}, lo = ms[m].s, hi = lo + ms[m].len;
+            int32_t d[QUAD] = {0, 0, 0, 0}, len[QUAD] = {0, 0, 0, 0}, lo = ms[m].s, hi = lo;
             const Member &head = ms[m];
+            bool ring = false;
             for (; m < ms.size() && ms[m].lat == head.lat && len[ms[m].i] == 0; m++) {
                 int32_t at = ms[m].s;
+                if (ms[m].len >= W) {
+                    len[ms[m].i] = QUAD_RING, ring = true;
+                    continue;
+                }
+                if (hi == lo) lo = at, hi = at + ms[m].len;
                 const int32_t want = lo + hi - ms[m].len; // (twice the start that centers it on the band so far)
                 while (2 * at - want > W) at -= W;
                 while (want - 2 * at > W) at += W;
@@ -303,11 +311,12 @@ void build_quads(const std::vector<int32_t> &off, const std::vector<int32_t> &ru
                 lo = nlo, hi = nhi;
                 d[ms[m].i] = at, len[ms[m].i] = ms[m].len;
             }
-            QuadBand q = {{head.lat, head.aux, ((lo % W) + W) % W, hi - lo, 0, 0, 0, 0}};
+            const int32_t length = ring ? std::max(std::max(hi - lo, W - 15), 1) : hi - lo;
+            QuadBand q = {{head.lat, head.aux, ((lo % W) + W) % W, length, 0, 0, 0, 0}};
             for (int i = 0; i < QUAD; i++)
-                if (len[i]) q.v[4 + i] = (d[i] - lo) << 16 | len[i];
+                if (len[i]) q.v[4 + i] = len[i] == QUAD_RING ? QUAD_RING : (d[i] - lo) << 16 | len[i];
             out->push_back(q);
-            work += (hi - lo + 15 + 31) / 32;
+            work += (length + 15 + 31) / 32;
         }
         groups->push_back({first / QUAD, first_band, (int32_t)out->size(), 0});
         steps.push_back(work);

@@ -3,17 +3,19 @@
 // A workgroup owns sixteen columns of four adjacent latitudes, a latitude per wavefront, and walks the bands of the other grid that any of them
 // sees (build_quads in s2attn_plan.cpp) in steps of 32 band positions: all four wavefronts stage the step's rows of two tensors, and those
 // whose latitude sees any of them work on them.  Position t of a band is column ws + w0 + t of its latitude; point c of the tile sees
-// t in [c + d, c + d + l).
+// t in [c + d, c + d + l), or t in [0, W) where its latitude sees the whole ring.
 //
 // Rows staged for 64 points, disk of radius R rings, arcs of a columns: (2 R + 4) (15 + a); with a latitude's 64 columns in the four wavefronts
 // (2 R + 1) (63 + a), in a ring of 128 (80) rows with two barriers a run.  Forward, dq and dk/dv took, us, that way / this way: 361x720 bf16 4 x 64
 // channels, R = 2: 269 / 267, 341 / 330, 369 / 326; 180x360 from 90x180 bf16 2 x 128 channels: 92 / 56, 98 / 68, 142 / 120; 128x256 fp32 4 x 32 channels
 // R = 4: 250 / 205, 252 / 220, 303 / 279; 91x180 bf16 forward alone, which is as long as its longest walk: 24 / 26.
+// Whole rings as such, in W positions: the last one 26.5 -> 24.5; 91x181 fp32 3 x 40 channels 77 -> 68, 75 -> 73, 106 -> 95.
 //
 // Two buffers, one barrier a step.  Bound by issue: vector instructions keep the SIMDs busy half the time, matrix instructions a tenth (16-bit) to a
 // quarter, at 3 to 5 wavefronts per SIMD, as registers allow.
 
-constexpr int QUAD = 4; // latitudes of a workgroup (= NW)
+constexpr int QUAD = 4;           // latitudes of a workgroup (= NW)
+constexpr int QUAD_RING = 0xffff; // (see build_quads)
 static_assert(QUAD == NW, "a latitude per wavefront");
 
 struct QuadUnit {
@@ -46,9 +48,12 @@ struct QuadStep {
     bool some;
     int pos;  // first position of its band
     int d, l; // what the wavefront's latitude sees of the band
+    bool ring;
     // does any point of the wavefront see any of the positions; do all see all
-    __device__ inline bool seen() const { return l > 0 && pos + HK > d && pos < d + l + HQ - 1; }
-    __device__ inline bool inner() const { return pos - d >= HQ - 1 && pos - d + HK <= l; }
+    __device__ inline bool seen() const { return l > 0 && pos + HK > d && pos < d + l + (ring ? 0 : HQ - 1); }
+    __device__ inline bool inner() const { return pos - d >= (ring ? 0 : HQ - 1) && pos - d + HK <= l; }
+    // point c sees position r of the step iff 0 <= first(c) + r < l
+    __device__ inline int first(int c) const { return pos - d - (ring ? 0 : c); }
 };
 
 // Where the walk's loads are: the step to fetch, and the band after its own, read while that is worked on.  All that a step loads, it loads in every
@@ -57,6 +62,7 @@ struct QuadStep {
 struct QuadWalk {
     const int *bands;
     int wv, word, zero; // word: lane % 8; zero: 0, in a vector register
+    int W;
     int band, end, pos;
     int lat, aux, ws, len, dl;
     int ahead; // int `word` of the band after
@@ -69,7 +75,7 @@ struct QuadWalk {
     }
     __device__ inline void start(const DArgs &a, const QuadUnit &u, int wv_, int lane)
     {
-        bands = a.q_bands, wv = wv_, word = lane & 7, zero = 0, end = u.last, pos = 0;
+        bands = a.q_bands, wv = wv_, word = lane & 7, zero = 0, W = a.Wi, end = u.last, pos = 0;
         asm("" : "+v"(zero));
         band = u.first - 1;
         read();
@@ -91,9 +97,13 @@ struct QuadWalk {
         }
         read();
     }
-    __device__ inline QuadStep step() const { return QuadStep{more(), pos, dl >> 16, dl & 0xffff}; }
+    __device__ inline QuadStep step() const
+    {
+        const bool ring = dl == QUAD_RING;
+        return QuadStep{more(), pos, ring ? 0 : dl >> 16, ring ? W : dl & 0xffff, ring};
+    }
     // first column of the step, in [0, W)
-    __device__ inline int column(int w0, int W) const
+    __device__ inline int column(int w0) const
     {
         int c = ws + w0 + pos;
         while (c >= W) c -= W;
