@@ -1,6 +1,8 @@
 """The bands that four latitudes share cover exactly the pairs of the CSR."""
 
 import ctypes
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -122,3 +124,20 @@ def test_a_header_that_points_outside_the_plan_is_refused():
         bad.header[_lib.PH["QUADS"]] = at
         assert lib.s2attn_diff_family(ctypes.byref(bad), ctypes.byref(shape), 16) == -1
         assert b"bands" in lib.s2attn_last_error()
+
+
+def test_a_plan_that_memory_does_not_hold_is_an_error():
+    """In a process of its own, whose memory is limited: an exception that left the C entry would end it."""
+    code = """
+import ctypes, resource
+from torch_harmonics_amd import _lib
+lib = _lib.load()
+col, off = (ctypes.c_int64 * 1)(0), (ctypes.c_int64 * 2)(0, 1)
+size = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize() + (256 << 20)
+resource.setrlimit(resource.RLIMIT_AS, (size, size))
+rc = lib.s2attn_plan_size(ctypes.cast(col, ctypes.c_void_p), ctypes.cast(off, ctypes.c_void_p), 1, 1, 1, 1 << 26, 2)
+assert rc == -2 and b"plan" in lib.s2attn_last_error(), (rc, lib.s2attn_last_error())
+print("refused")
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "refused" in out.stdout, out.stderr[-500:]

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <exception>
 #include <numeric>
 #include <vector>
 
@@ -474,33 +475,51 @@ int build_blob(const int64_t *col_idx, const int64_t *row_off, int64_t nnz, int 
 
 } // namespace
 
+namespace {
+// An exception (memory) must not leave a C entry.
+template <typename F> int64_t guarded(F f)
+{
+    try {
+        return f();
+    } catch (const std::exception &e) {
+        return s2attn_fail(S2ATTN_E_UNSUPPORTED, "plan: %s", e.what());
+    }
+}
+} // namespace
+
 extern "C" int64_t s2attn_plan_count(const int64_t *col_idx, const int64_t *row_off, int64_t nnz, int nlat_in, int nlon_in,
                                      int nlat_out, int nlon_out)
 {
-    int64_t n = 0;
-    const int rc = decompose(col_idx, row_off, nnz, nlat_in, nlon_in, nlat_out, nlon_out, nullptr, &n);
-    return rc == S2ATTN_OK ? n : (int64_t)rc;
+    return guarded([&]() -> int64_t {
+        int64_t n = 0;
+        const int rc = decompose(col_idx, row_off, nnz, nlat_in, nlon_in, nlat_out, nlon_out, nullptr, &n);
+        return rc == S2ATTN_OK ? n : (int64_t)rc;
+    });
 }
 
 extern "C" int64_t s2attn_plan_size(const int64_t *col_idx, const int64_t *row_off, int64_t nnz, int nlat_in, int nlon_in,
                                     int nlat_out, int nlon_out)
 {
-    std::vector<int32_t> blob;
-    const int rc = build_blob(col_idx, row_off, nnz, nlat_in, nlon_in, nlat_out, nlon_out, blob);
-    return rc == S2ATTN_OK ? (int64_t)blob.size() : (int64_t)rc;
+    return guarded([&]() -> int64_t {
+        std::vector<int32_t> blob;
+        const int rc = build_blob(col_idx, row_off, nnz, nlat_in, nlon_in, nlat_out, nlon_out, blob);
+        return rc == S2ATTN_OK ? (int64_t)blob.size() : (int64_t)rc;
+    });
 }
 
 extern "C" int s2attn_plan_build(const int64_t *col_idx, const int64_t *row_off, int64_t nnz, int nlat_in, int nlon_in,
                                  int nlat_out, int nlon_out, int32_t *blob_out, int64_t blob_ints)
 {
     if (!blob_out) return s2attn_fail(S2ATTN_E_INVALID, "plan output buffer is null");
-    std::vector<int32_t> blob;
-    const int rc = build_blob(col_idx, row_off, nnz, nlat_in, nlon_in, nlat_out, nlon_out, blob);
-    if (rc != S2ATTN_OK) return rc;
-    if ((int64_t)blob.size() != blob_ints)
-        return s2attn_fail(S2ATTN_E_INVALID, "the plan of this CSR has %zu ints, the buffer %lld (size it with s2attn_plan_size)", blob.size(), (long long)blob_ints);
-    std::copy(blob.begin(), blob.end(), blob_out);
-    return S2ATTN_OK;
+    return (int)guarded([&]() -> int64_t {
+        std::vector<int32_t> blob;
+        const int rc = build_blob(col_idx, row_off, nnz, nlat_in, nlon_in, nlat_out, nlon_out, blob);
+        if (rc != S2ATTN_OK) return rc;
+        if ((int64_t)blob.size() != blob_ints)
+            return s2attn_fail(S2ATTN_E_INVALID, "the plan of this CSR has %zu ints, the buffer %lld (size it with s2attn_plan_size)", blob.size(), (long long)blob_ints);
+        std::copy(blob.begin(), blob.end(), blob_out);
+        return S2ATTN_OK;
+    });
 }
 
 // Regrouped psi for the ring-step kernels (see include/s2attn.h): a stable counting sort of the CSR entries by the
